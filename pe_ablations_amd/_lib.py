@@ -1,4 +1,4 @@
-"""ctypes binding of libpe_attn.so (include/pe_attn.h).
+"""ctypes binding of libpe_attn.so (include/pe_attn.h, include/pe_vocab.h).
 
 The library is loaded lazily from this package directory.  There is no fallback: when the library
 is missing every entry point raises, so a run can never silently compute on another path.
@@ -36,6 +36,15 @@ EXPORTED = [
     "pe_attn_bwd_masked", "pe_attn_bwd_masked_workspace_bytes",
 ]
 
+# every symbol include/pe_vocab.h declares
+EXPORTED_VOCAB = [
+    "pe_embed_fwd", "pe_embed_bwd_workspace_bytes", "pe_embed_bwd", "pe_loss_check", "pe_loss_workspace_bytes",
+    "pe_loss_stats_floats", "pe_loss_fwd", "pe_loss_bwd", "pe_loss_step",
+]
+
+PE_LOSS_NONE, PE_LOSS_SUM, PE_LOSS_MEAN = 0, 1, 2
+PE_LOSS_MAX_TOP_K = 1024
+
 # kernel stages bracketed by pe_attn_set_stage_events
 STAGES = ["fwd_prep", "fwd_core", "bwd_pre", "bwd_dkdv", "bwd_dq", "bwd_inv"]
 
@@ -60,6 +69,15 @@ class PeParams(ctypes.Structure):
 class PeNormParams(ctypes.Structure):
     _fields_ = [("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
                 ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class PeLossParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "row_stride", "grad_row_stride", "shift", "ignore_index",
+                                              "teacher_id_stride", "teacher_row_stride")] + \
+               [(n, ctypes.c_int32) for n in ("vocab", "dtype", "label_bytes", "reduction", "top_k", "teacher_dtype",
+                                              "teacher_id_bytes")] + \
+               [(n, ctypes.c_float) for n in ("hard_weight", "soft_weight", "temperature", "grad_factor")] + \
+               [("reserved", ctypes.c_int32)]
 
 
 _lib = None
@@ -149,6 +167,25 @@ def lib():
             L.pe_attn_decode.restype = ctypes.c_int
             L.pe_attn_set_stage_events.argtypes = [vp]
             L.pe_attn_set_stage_events.restype = ctypes.c_int
+            L.pe_embed_fwd.argtypes = [vp, i32, i64, vp, i32, i64, i32, i64, ctypes.c_float, vp, i64, vp]
+            L.pe_embed_fwd.restype = ctypes.c_int
+            L.pe_embed_bwd_workspace_bytes.argtypes = [i64, i64, i32]
+            L.pe_embed_bwd_workspace_bytes.restype = sz
+            L.pe_embed_bwd.argtypes = [vp, i32, i64, vp, i32, i64, i64, i32, ctypes.c_float, i64, vp, i64, vp, sz, vp]
+            L.pe_embed_bwd.restype = ctypes.c_int
+            LP = ctypes.POINTER(PeLossParams)
+            L.pe_loss_check.argtypes = [LP]
+            L.pe_loss_check.restype = ctypes.c_int
+            L.pe_loss_workspace_bytes.argtypes = [LP]
+            L.pe_loss_workspace_bytes.restype = sz
+            L.pe_loss_stats_floats.argtypes = [LP]
+            L.pe_loss_stats_floats.restype = i64
+            L.pe_loss_fwd.argtypes = [LP, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+            L.pe_loss_fwd.restype = ctypes.c_int
+            L.pe_loss_bwd.argtypes = [LP, vp, vp, vp, vp, vp, vp, vp, vp]
+            L.pe_loss_bwd.restype = ctypes.c_int
+            L.pe_loss_step.argtypes = [LP, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+            L.pe_loss_step.restype = ctypes.c_int
             _lib = L
     return _lib
 

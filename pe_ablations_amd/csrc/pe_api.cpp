@@ -320,6 +320,8 @@ pe::CoreArgs core_args(const pe_attn_params* p, const Layout& L, const char* ws,
 
 }  // namespace
 
+int pe::device_ready() { return device_ok(); }
+
 extern "C" {
 
 int pe_attn_version(void) { return PE_ATTN_ABI_VERSION; }

@@ -291,4 +291,41 @@ struct ReduceArgs {
 };
 int launch_reduce(const ReduceArgs& a, hipStream_t s);
 
+// 0 when the current device is a gfx950, else PE_ERR_NO_DEVICE (pe_api.cpp)
+int device_ready();
+
+// The losses over the vocabulary (include/pe_vocab.h).  `phase` of launch_loss: the row statistics and losses,
+// the gradient from kept statistics, or both from one read of the logits.
+struct LossArgs {
+  const void* z; int64_t z_rs;
+  void* dz; int64_t dz_rs;
+  const void* labels; int label_bytes; int64_t shift, ignore;
+  const void* tid; int64_t tid_rs; int tid_bytes;
+  const void* tlog; int64_t tlog_rs; int tlog_dtype;
+  int64_t rows; int V, K, reduction;
+  float hw, sw, T, factor;
+  float* row_loss;        // one per row
+  float* stats;           // [rows][3]: maximum, sum, sum at the temperature; [3 rows]: 1 / rows that count
+  const float* dloss;     // one, or one per row (PE_LOSS_NONE)
+  const float* inv_count; // 1 / rows that count (PE_LOSS_MEAN)
+};
+enum { LOSS_FWD = 0, LOSS_BWD = 1, LOSS_STEP = 2 };
+int launch_loss(int dtype, int phase, const LossArgs& a, hipStream_t s);
+// 1 / rows that count (PE_LOSS_MEAN) from the labels
+int launch_loss_count(const LossArgs& a, float* inv_count, hipStream_t s);
+// the sum or mean of row_loss; also 1 / rows that count when inv_count is not NULL
+int launch_loss_reduce(const LossArgs& a, float* loss, float* inv_count, hipStream_t s);
+
+// The scaled token embedding and its gradient
+struct EmbedArgs {
+  const void* ids; int id_bytes; int64_t n;
+  const void* x; int64_t x_rs;  // the weight, or the gradient of the looked-up rows
+  void* y; int64_t y_rs;        // the looked-up rows, or the gradient of the weight
+  int64_t V; int H; float scale; int64_t pad;
+  int32_t *key, *order;         // the tokens sorted by id: their ids and positions
+};
+int launch_embed_fwd(int dtype, const EmbedArgs& a, hipStream_t s);
+int64_t embed_bwd_workspace(int64_t n, int64_t V, int H);
+int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s);
+
 }  // namespace pe

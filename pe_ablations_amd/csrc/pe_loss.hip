@@ -1,0 +1,285 @@
+// Losses over the vocabulary (include/pe_vocab.h): next-token cross entropy and distillation from a teacher's
+// top logits, forward, backward, and both from one read of the logits.
+//
+// With m = max z, s = sum exp(z - m) and s_T = sum exp((z - m) / T) of a row,
+//     hard = (m - z_y) + ln s
+//     soft = T^2 sum_k p_k (ln p_k + (m - z_k) / T + ln s_T)
+//     dz_j = c (hw e^(z_j - m) / s + sw T P e^((z_j - m) / T) / s_T),  P = sum_k p_k (1, or 0 with no pair present)
+// and at the at most K + 1 places that the label and the teacher name, dz_j less c hw [j = y] and
+// c sw T sum_{k: id_k = j} p_k.  A workgroup takes a row; those few places are written again behind the dense
+// ones, by one thread for each different id.
+#include "pe_common.h"
+#include "pe_internal.h"
+#include "pe_vocab.h"
+
+namespace pe {
+
+namespace {
+
+template <int DT> __device__ __forceinline__ float elem(const void* p, int64_t i) {
+  if constexpr (DT == 1) return ((const float*)p)[i];
+  else if constexpr (DT == 0) return bf2f(((const uint16_t*)p)[i]);
+  else return h2f(((const uint16_t*)p)[i]);
+}
+template <int DT> __device__ __forceinline__ void put(void* p, int64_t i, float x) {
+  if constexpr (DT == 1) ((float*)p)[i] = x;
+  else if constexpr (DT == 0) ((uint16_t*)p)[i] = f2bf(x);
+  else ((uint16_t*)p)[i] = f2h(x);
+}
+
+__device__ __forceinline__ int64_t load_id(const void* p, int bytes, int64_t i) {
+  return bytes == 8 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+// the row's label; false when the row does not count.  Without labels every row counts, with label -1
+__device__ __forceinline__ bool row_label(const LossArgs& a, int64_t r, int64_t& y) {
+  y = -1;
+  if (!a.labels) return true;
+  if (a.shift) {
+    if (r % a.shift == a.shift - 1) return false;
+    r += 1;
+  }
+  y = load_id(a.labels, a.label_bytes, r);
+  return y != a.ignore;
+}
+
+// a maximum and the sums of exponentials relative to it; -inf and no sums to begin with
+struct Stat { float m, s, t; };
+
+// two of them as one.  A maximum of -inf is no reference (its differences would be NaN): 0 is taken then, relative to
+// which its exponentials are 0 as well
+template <bool HARD, bool SOFT> __device__ __forceinline__ Stat join(const Stat& x, const Stat& y, float lt) {
+  Stat r;
+  r.m = fmaxf(x.m, y.m);
+  const float ref = r.m == -INFINITY ? 0.f : r.m;
+  r.s = HARD ? x.s * exp2f((x.m - ref) * LOG2E) + y.s * exp2f((y.m - ref) * LOG2E) : 0.f;
+  r.t = SOFT ? x.t * exp2f((x.m - ref) * lt) + y.t * exp2f((y.m - ref) * lt) : 0.f;
+  return r;
+}
+
+template <int T> __device__ __forceinline__ float block_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float r = red[0];
+  for (int i = 1; i < T / 64; ++i) r += red[i];
+  return r;
+}
+template <int T> __device__ __forceinline__ float block_max(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float r = red[0];
+  for (int i = 1; i < T / 64; ++i) r = fmaxf(r, red[i]);
+  return r;
+}
+
+}  // namespace
+
+template <int DT, int PHASE, bool HARD, bool SOFT, int T>
+__global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
+  __shared__ float red[T / 64];
+  __shared__ Stat wred[T / 64];
+  __shared__ int32_t tid_l[SOFT ? PE_LOSS_MAX_TOP_K : 1];  // the teacher's ids, -1 where absent
+  __shared__ float tp_l[SOFT ? PE_LOSS_MAX_TOP_K : 1];     // and probabilities
+  const int64_t r = blockIdx.x;
+  const int t = threadIdx.x, V = a.V;
+  constexpr int ES = DT == 1 ? 4 : 2;
+  const char* z = (const char*)a.z + r * a.z_rs * ES;
+  char* dz = PHASE == LOSS_FWD ? nullptr : (char*)a.dz + r * a.dz_rs * ES;
+  int64_t y;
+  if (!row_label(a, r, y)) {
+    if (PHASE != LOSS_FWD)
+      for (int j = t; j < V; j += T) put<DT>(dz, j, 0.f);
+    if (t == 0) {
+      if (PHASE != LOSS_BWD) a.row_loss[r] = 0.f;
+      if (PHASE == LOSS_FWD && a.stats) a.stats[3 * r] = a.stats[3 * r + 1] = a.stats[3 * r + 2] = 0.f;
+    }
+    return;
+  }
+  const bool bad = a.labels && (y < 0 || y >= V);
+  const float lt = LOG2E / a.T;
+
+  Stat st{-INFINITY, 0.f, 0.f};
+  if (PHASE == LOSS_BWD) {
+    st = Stat{a.stats[3 * r], a.stats[3 * r + 1], a.stats[3 * r + 2]};
+  } else {
+    for (int j = t; j < V; j += T) {
+      const float x = elem<DT>(z, j);
+      if (x > st.m) {
+        if (HARD) st.s *= exp2f((st.m - x) * LOG2E);
+        if (SOFT) st.t *= exp2f((st.m - x) * lt);
+        st.m = x;
+      }
+      const float ref = st.m == -INFINITY ? 0.f : st.m;
+      if (HARD) st.s += exp2f((x - ref) * LOG2E);
+      if (SOFT) st.t += exp2f((x - ref) * lt);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+      st = join<HARD, SOFT>(st, Stat{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)}, lt);
+    if ((t & 63) == 0) wred[t >> 6] = st;
+    __syncthreads();
+    st = wred[0];
+    for (int i = 1; i < T / 64; ++i) st = join<HARD, SOFT>(st, wred[i], lt);
+    if (PHASE == LOSS_FWD && a.stats && t == 0) {
+      a.stats[3 * r] = st.m;
+      a.stats[3 * r + 1] = st.s;
+      a.stats[3 * r + 2] = st.t;
+    }
+  }
+
+  // the teacher's probabilities
+  float P = 0.f;
+  if (SOFT) {
+    float mx = -INFINITY;
+    for (int k = t; k < a.K; k += T) {
+      const int64_t id = load_id(a.tid, a.tid_bytes, r * a.tid_rs + k);
+      const float x = load_as_float(a.tlog, r * a.tlog_rs + k, a.tlog_dtype);
+      const bool have = id >= 0 && id < V && x != -INFINITY;
+      tid_l[k] = have ? (int32_t)id : -1;
+      tp_l[k] = x;
+      if (have) mx = fmaxf(mx, x);
+    }
+    mx = block_max<T>(mx, red);
+    float n = 0.f;
+    for (int k = t; k < a.K; k += T)
+      if (tid_l[k] >= 0) n += exp2f((tp_l[k] - mx) * lt);
+    n = block_sum<T>(n, red);
+    P = n != 0.f ? 1.f : 0.f;
+    float sum = 0.f;
+    for (int k = t; k < a.K; k += T) {
+      float p = 0.f;
+      if (tid_l[k] >= 0) {
+        const float d = tp_l[k] - mx;
+        p = exp2f(d * lt) / n;
+        if (PHASE != LOSS_BWD && p != 0.f)
+          sum += p * ((d + st.m - elem<DT>(z, tid_l[k])) / a.T - logf(n) + logf(st.t));
+      }
+      tp_l[k] = p;
+    }
+    if (PHASE != LOSS_BWD) {
+      sum = block_sum<T>(sum, red);
+      P = n != 0.f ? 1.f : 0.f;
+      if (t == 0) {
+        float loss = a.sw * a.T * a.T * sum;
+        if (HARD) loss += a.hw * (bad ? NAN : (st.m - elem<DT>(z, y)) + logf(st.s));
+        a.row_loss[r] = bad ? NAN : loss;
+      }
+    }
+    __syncthreads();
+  } else if (PHASE != LOSS_BWD && t == 0) {
+    a.row_loss[r] = bad ? NAN : a.hw * ((st.m - elem<DT>(z, y)) + logf(st.s));
+  }
+
+  if (PHASE == LOSS_FWD) return;
+  float c = a.factor;
+  if (a.dloss) c *= a.dloss[a.reduction == PE_LOSS_NONE ? r : 0];
+  if (a.inv_count) c *= *a.inv_count;
+  if (bad) c = NAN;
+  const float ref = st.m;
+  const float ch = HARD ? c * a.hw / st.s : 0.f, ct = SOFT ? c * a.sw * a.T * P / st.t : 0.f;
+  auto dense = [&](float x) {
+    float g = 0.f;
+    if (HARD) g += ch * exp2f((x - ref) * LOG2E);
+    if (SOFT) g += ct * exp2f((x - ref) * lt);
+    return g;
+  };
+  for (int j = t; j < V; j += T) put<DT>(dz, j, dense(elem<DT>(z, j)));
+  __syncthreads();
+  // the named places again, by the first of the pairs with an id; the label's by thread 0 unless a pair has it
+  if (SOFT) {
+    for (int k = t; k < a.K; k += T) {
+      const int32_t id = tid_l[k];
+      if (id < 0) continue;
+      float p = 0.f;
+      bool first = true;
+      for (int i = 0; i < a.K; ++i) {
+        if (tid_l[i] == id) {
+          first = first && i >= k;
+          p += tp_l[i];
+        }
+      }
+      if (!first) continue;
+      float g = dense(elem<DT>(z, id)) - c * a.sw * a.T * p;
+      if (HARD && id == y) g -= c * a.hw;
+      put<DT>(dz, id, g);
+    }
+  }
+  if (HARD && t == 0 && !bad) {
+    bool named = false;
+    if (SOFT)
+      for (int i = 0; i < a.K; ++i) named |= tid_l[i] == y;
+    if (!named) put<DT>(dz, y, dense(elem<DT>(z, y)) - c * a.hw);
+  }
+}
+
+// 1 / rows that count, and the sum or mean of the row losses: one workgroup, thread t taking rows t, t + 1024, ...
+template <bool SUM>
+__global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* loss, float* inv_count) {
+  __shared__ double rs[16];
+  __shared__ int32_t rn[16];
+  const int t = threadIdx.x;
+  double s = 0.;
+  int32_t n = 0;
+  for (int64_t r = t; r < a.rows; r += 1024) {
+    int64_t y;
+    if (SUM) s += a.row_loss[r];
+    n += row_label(a, r, y) ? 1 : 0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    if (SUM) s += __shfl_xor(s, o, 64);
+    n += __shfl_xor(n, o, 64);
+  }
+  if ((t & 63) == 0) {
+    rs[t >> 6] = s;
+    rn[t >> 6] = n;
+  }
+  __syncthreads();
+  if (t != 0) return;
+  for (int i = 1; i < 16; ++i) {
+    s += rs[i];
+    n += rn[i];
+  }
+  if (SUM) *loss = (float)(a.reduction == PE_LOSS_MEAN ? s / (double)n : s);
+  if (inv_count) *inv_count = 1.f / (float)n;
+}
+
+template <int DT, int PHASE> static int run_loss(const LossArgs& a, hipStream_t s) {
+  constexpr int T = 256;
+  const dim3 grid((unsigned)a.rows), block(T);
+  if (a.sw == 0.f) hipLaunchKernelGGL((loss_row_kernel<DT, PHASE, true, false, T>), grid, block, 0, s, a);
+  else if (a.hw == 0.f) hipLaunchKernelGGL((loss_row_kernel<DT, PHASE, false, true, T>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((loss_row_kernel<DT, PHASE, true, true, T>), grid, block, 0, s, a);
+  return hipGetLastError() == hipSuccess ? 0 : -7;
+}
+
+template <int DT> static int loss_phase(int phase, const LossArgs& a, hipStream_t s) {
+  if (phase == LOSS_FWD) return run_loss<DT, LOSS_FWD>(a, s);
+  if (phase == LOSS_BWD) return run_loss<DT, LOSS_BWD>(a, s);
+  return run_loss<DT, LOSS_STEP>(a, s);
+}
+
+int launch_loss(int dtype, int phase, const LossArgs& a, hipStream_t s) {
+  if (a.rows == 0) return 0;
+  if (dtype == 0) return loss_phase<0>(phase, a, s);
+  if (dtype == 1) return loss_phase<1>(phase, a, s);
+  return loss_phase<2>(phase, a, s);
+}
+
+int launch_loss_count(const LossArgs& a, float* inv_count, hipStream_t s) {
+  hipLaunchKernelGGL(loss_reduce_kernel<false>, dim3(1), dim3(1024), 0, s, a, (float*)nullptr, inv_count);
+  return hipGetLastError() == hipSuccess ? 0 : -7;
+}
+
+int launch_loss_reduce(const LossArgs& a, float* loss, float* inv_count, hipStream_t s) {
+  hipLaunchKernelGGL(loss_reduce_kernel<true>, dim3(1), dim3(1024), 0, s, a, loss, inv_count);
+  return hipGetLastError() == hipSuccess ? 0 : -7;
+}
+
+}  // namespace pe

@@ -1,19 +1,138 @@
 """Drop-in for src/model/embeddings.py: TokenEmbedding (parameter ``embedding.weight``), whose
-weight the Transformer ties to its output projection (src/model/embeddings.py:7-34)."""
+weight the Transformer ties to its output projection (src/model/embeddings.py:7-34), and the scaled
+lookup ``embedding`` behind its ``scale``: HIP kernels, forward (pe_embed_fwd) and the weight's
+gradient (pe_embed_bwd), which sorts the tokens by id and adds each id's rows in order.
+"""
+
+from typing import Optional
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
+
+from . import _lib
+from .functional import _dtype_code, _expression_grads, _on, _stream, plain_autograd
+
+_FLOATS = (torch.bfloat16, torch.float32, torch.float16)
+_MAX_TOKENS = 1 << 24
+
+
+def _check(ids: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[int]) -> int:
+    """The checks of an embedding call; padding_idx as the C ABI takes it (-1 for none)."""
+    if not weight.is_cuda:
+        raise RuntimeError("embedding runs on the GPU only (got a CPU weight)")
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"embedding: weight must be (vocab, dim), got shape {tuple(weight.shape)}")
+    if weight.dtype not in _FLOATS:
+        raise TypeError(f"embedding supports bf16 / fp16 / fp32 weights, got {weight.dtype}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
+    if ids.device != weight.device:
+        raise ValueError(f"embedding: ids are on {ids.device}, the weight on {weight.device}")
+    if padding_idx is None:
+        return -1
+    V = weight.shape[0]
+    if not -V <= padding_idx < V:
+        raise ValueError(f"embedding: padding_idx {padding_idx} is outside a vocabulary of {V}")
+    return padding_idx % V
+
+
+def _lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    V, H = weight.shape
+    if weight.stride(1) != 1 or weight.stride(0) < H:
+        weight = weight.contiguous()
+    ids = ids.contiguous()
+    out = torch.empty(ids.shape + (H,), dtype=weight.dtype, device=weight.device)
+    n = ids.numel()
+    if n:
+        dev = weight.device
+        with _on(dev):
+            rc = _lib.lib().pe_embed_fwd(ids.data_ptr(), ids.element_size(), n, weight.data_ptr(),
+                                         _dtype_code(weight.dtype), V, H, weight.stride(0), scale, out.data_ptr(), H,
+                                         _stream(dev))
+        _lib.check(rc)
+    return out
+
+
+def embedding_backward(ids: torch.Tensor, dy: torch.Tensor, vocab_size: int, *, scale: float = 1.0,
+                       padding_idx: Optional[int] = None) -> torch.Tensor:
+    """The weight gradient (vocab_size, dim) of ``embedding(ids, weight, scale=scale)`` for the upstream
+    gradient dy (*ids.shape, dim), in dy's dtype: scale times the sum of each id's rows, in the order of the
+    tokens, in fp32 (bitwise reproducible).  padding_idx's row is 0; ids outside the vocabulary add nothing."""
+    if not dy.is_cuda:
+        raise RuntimeError("embedding_backward runs on the GPU only (got a CPU tensor)")
+    if tuple(dy.shape[:-1]) != tuple(ids.shape) or dy.dim() != ids.dim() + 1:
+        raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} must be ids {tuple(ids.shape)} plus a last dim")
+    H = dy.shape[-1]
+    n = ids.numel()
+    if n > _MAX_TOKENS:
+        raise ValueError(f"embedding_backward: {n} tokens in one call, at most {_MAX_TOKENS} are supported")
+    dev = dy.device
+    dw = torch.empty((vocab_size, H), dtype=dy.dtype, device=dev)
+    pad = _check(ids, dw, padding_idx)
+    dy = dy.reshape(-1, H)
+    if dy.stride(1) != 1 or dy.stride(0) < H:
+        dy = dy.contiguous()
+    ids = ids.contiguous()
+    L = _lib.lib()
+    nb = L.pe_embed_bwd_workspace_bytes(n, vocab_size, H)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = L.pe_embed_bwd(ids.data_ptr(), ids.element_size(), n, dy.data_ptr(), _dtype_code(dy.dtype),
+                            max(dy.stride(0), H), vocab_size, H, scale, pad, dw.data_ptr(), H, ws.data_ptr(), nb,
+                            _stream(dev))
+    _lib.check(rc)
+    return dw
+
+
+class EmbeddingFn(torch.autograd.Function):
+    """The lookup with pe_embed_bwd as its backward; under create_graph and with batched gradients the
+    backward differentiates F.embedding(ids, weight) * scale (as RMSNormFn)."""
+
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx):
+        ctx.save_for_backward(weight, ids)
+        ctx.scale, ctx.padding_idx = scale, padding_idx
+        return _lookup(ids, weight, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        weight, ids = ctx.saved_tensors
+        if torch.is_grad_enabled() or not plain_autograd(dy):
+            return _expression_grads(lambda: F.embedding(ids, weight, ctx.padding_idx) * ctx.scale, (weight,), ctx,
+                                     dy) + (None, None, None)
+        return embedding_backward(ids, dy, weight.shape[0], scale=ctx.scale, padding_idx=ctx.padding_idx), None, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+              padding_idx: Optional[int] = None) -> torch.Tensor:
+    """weight[ids] * scale, (*ids.shape, dim) in the weight's dtype, the product in fp32 and rounded once.
+    weight (vocab, dim) bf16 / fp16 / fp32 on the GPU, ids int64 / int32 on the same device.  Differentiable in
+    the weight (embedding_backward); the rows of padding_idx get no gradient.  An id outside the vocabulary
+    cannot be refused without waiting for the GPU: its row is NaN."""
+    pad = _check(ids, weight, padding_idx)
+    if torch.is_grad_enabled() and weight.requires_grad:
+        if ids.numel() > _MAX_TOKENS:
+            raise ValueError(f"embedding: {ids.numel()} tokens in one call with gradients, at most {_MAX_TOKENS}")
+        return EmbeddingFn.apply(weight, ids, float(scale), None if pad < 0 else pad)
+    return _lookup(ids, weight, float(scale))
 
 
 class TokenEmbedding(nn.Module):
-    def __init__(self, vocab_size: int, embed_dim: int):
+    """``scale`` (an addition; default None = the reference's plain lookup through torch): the rows times this
+    factor, sqrt(embed_dim) in models that tie the weight to an output projection, through ``embedding``."""
+
+    def __init__(self, vocab_size: int, embed_dim: int, scale: Optional[float] = None):
         super().__init__()
         self.vocab_size = vocab_size
         self.embed_dim = embed_dim
+        self.scale = scale
         self.embedding = nn.Embedding(vocab_size, embed_dim)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return self.embedding(x)
+        if self.scale is None:
+            return self.embedding(x)
+        return embedding(x, self.embedding.weight, scale=self.scale)
 
     @property
     def weight(self) -> torch.Tensor:

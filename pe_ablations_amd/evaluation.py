@@ -46,9 +46,9 @@ _CONFIG_KEYS = {
 }
 
 
-# read in addition: both only turn loads the reference script would reject (a state dict that does
-# not fit its model) into working ones, and leave every load it accepts unchanged
-_EXTRA_KEYS = {"ffn_dim": None, "pope_fused": False}
+# read in addition: fields whose checkpoints the reference script would reject (a state dict that does
+# not fit its model) or that its trainer does not write, so every load it accepts stays unchanged
+_EXTRA_KEYS = {"ffn_dim": None, "pope_fused": False, "embedding_scale": None, "fused_loss": False}
 
 
 def config_from_checkpoint(checkpoint: dict) -> TransformerConfig:

@@ -7,10 +7,13 @@ checkpoint written by the reference's trainer loads with ``load_state_dict`` unc
 (src/model/transformer.py:109-301).  The attention of every layer is the library's fused HIP
 kernel; the projections, norms, SwiGLU and the LM head are torch ops (hipBLASLt GEMMs).
 
-One addition: ``pope_fused`` (default False).  When True, pe_mode "pope" / "pope_floor" layers use
+Additions: ``pope_fused`` (default False).  When True, pe_mode "pope" / "pope_floor" layers use
 the fused form of the legacy API, all ``head_dim`` dims PoPE-encoded with no content half (the
 shape of the 1B long-context configuration), instead of the reference's content + ``pope_d_rope``
-split.
+split.  ``embedding_scale`` (default None) multiplies the token embedding by a factor, and
+``fused_loss`` (default False) computes the next-token loss with the library's kernels instead of
+F.cross_entropy on a shifted copy of the logits; with a teacher's top logits, ``forward`` returns the
+distillation loss (both from ``losses``).
 """
 
 from __future__ import annotations
@@ -27,6 +30,7 @@ from .embeddings import TokenEmbedding
 from .ffn import FeedForward
 from .fpope import FoPEPoPEEmbedding
 from .fpope_attention import FPoPEGroupedQueryAttentionWithCache
+from .losses import cross_entropy, distillation_loss
 from .normalization import RMSNorm
 from .pope import PoPEEmbedding
 from .rope import NTKAwareRotaryEmbedding, RotaryEmbedding, YaRNRotaryEmbedding
@@ -34,7 +38,8 @@ from .rope import NTKAwareRotaryEmbedding, RotaryEmbedding, YaRNRotaryEmbedding
 
 @dataclass
 class TransformerConfig:
-    """Fields and defaults of src/model/transformer.py:21-106, plus ``pope_fused``."""
+    """Fields and defaults of src/model/transformer.py:21-106, plus ``pope_fused``, ``embedding_scale`` and
+    ``fused_loss``."""
 
     vocab_size: int = 50257
     hidden_dim: int = 512
@@ -73,6 +78,9 @@ class TransformerConfig:
     dropout: float = 0.0
     tie_embeddings: bool = True
     gradient_checkpointing: bool = False
+
+    embedding_scale: Optional[float] = None
+    fused_loss: bool = False
 
     def __post_init__(self) -> None:
         if self.head_dim is None:
@@ -155,7 +163,7 @@ class Transformer(nn.Module):
     def __init__(self, config: TransformerConfig):
         super().__init__()
         self.config = config
-        self.token_embedding = TokenEmbedding(config.vocab_size, config.hidden_dim)
+        self.token_embedding = TokenEmbedding(config.vocab_size, config.hidden_dim, scale=config.embedding_scale)
         self.rope = None
         self.fpope = None
         self.pope = None
@@ -208,11 +216,18 @@ class Transformer(nn.Module):
                 torch.nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
-                start_pos: int = 0, use_cache: bool = False) -> dict:
+                start_pos: int = 0, use_cache: bool = False,
+                teacher: Optional[tuple[torch.Tensor, torch.Tensor]] = None, temperature: float = 1.0,
+                soft_weight: float = 0.5) -> dict:
         """{'logits'} and, with ``labels``, {'loss'}: next-token cross entropy over the shifted
         sequence with ignore_index -100 (src/model/transformer.py:313-364).  ``use_cache``
         (an addition) feeds the tokens at absolute positions start_pos.. through
-        every layer's KV cache, which must hold exactly start_pos earlier rows."""
+        every layer's KV cache, which must hold exactly start_pos earlier rows.  ``teacher`` (an
+        addition, with ``labels``) = (ids, logits), both (B, S, K): a teacher model's top logits at every
+        position; the loss is then ``losses.distillation_loss`` over the shifted sequence at this
+        ``temperature`` and ``soft_weight``."""
+        if teacher is not None and labels is None:
+            raise ValueError("a teacher needs labels: they say which positions the loss counts")
         x = self.token_embedding(input_ids)
         for layer in self.layers:
             if self.gradient_checkpointing and self.training:
@@ -222,7 +237,12 @@ class Transformer(nn.Module):
         x = self.norm(x)
         logits = self.output(x)
         out = {"logits": logits}
-        if labels is not None:
+        if teacher is not None:
+            out["loss"] = distillation_loss(logits, labels, teacher[0], teacher[1], temperature=temperature,
+                                            soft_weight=soft_weight, shift=True)
+        elif labels is not None and self.config.fused_loss:
+            out["loss"] = cross_entropy(logits, labels, shift=True)
+        elif labels is not None:
             shift_logits = logits[..., :-1, :].contiguous()
             shift_labels = labels[..., 1:].contiguous()
             out["loss"] = F.cross_entropy(shift_logits.view(-1, self.config.vocab_size), shift_labels.view(-1),
