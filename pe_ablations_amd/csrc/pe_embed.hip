@@ -2,9 +2,17 @@
 //
 //     out[t] = weight[ids[t]] * scale        dweight[v] = scale * sum_{t: ids[t] = v} dy[t]
 //
-// Both are bound by memory.  The gradient sorts the tokens by id first (an int32 key and position each), then
-// every row of the vocabulary finds its run of tokens by binary search and adds their rows in order, so each row
-// of the gradient is written once, by one workgroup, and no sum depends on the order in which workgroups run.
+// Both are bound by memory.  The gradient sorts the tokens by id (stable, so each id's tokens stay in order), notes
+// each id's run of tokens and sums whole chunks of sorted tokens that share one id ahead of time, and then adds up
+// the run of every row of the vocabulary: each row of the gradient is written once, by one workgroup, rows without a
+// token as zeros, and no sum depends on the order in which workgroups run.
+//
+// A row of H elements is cut into pieces of VB bytes, the largest of 16, 8, 4 and 2 that the row length, the strides
+// and the addresses allow, a piece a lane; `lpr` lanes (a power of two) work on a row together, 256 / lpr rows at
+// once in a workgroup, and rows longer than lpr pieces are cut into column slices.
+#include <algorithm>
+#include <type_traits>
+
 #include "pe_common.h"
 #include "pe_internal.h"
 
@@ -12,16 +20,54 @@ namespace pe {
 
 namespace {
 
-template <int DT> __device__ __forceinline__ float elem(const void* p, int64_t i) {
-  if constexpr (DT == 1) return ((const float*)p)[i];
-  else if constexpr (DT == 0) return bf2f(((const uint16_t*)p)[i]);
-  else return h2f(((const uint16_t*)p)[i]);
-}
-template <int DT> __device__ __forceinline__ void put(void* p, int64_t i, float x) {
-  if constexpr (DT == 1) ((float*)p)[i] = x;
-  else if constexpr (DT == 0) ((uint16_t*)p)[i] = f2bf(x);
-  else ((uint16_t*)p)[i] = f2h(x);
-}
+template <int VB> struct Raw;
+template <> struct Raw<16> { using T = u32x4; };
+template <> struct Raw<8> { using T = u32x2; };
+template <> struct Raw<4> { using T = uint32_t; };
+template <> struct Raw<2> { using T = uint16_t; };
+
+// a piece of VB bytes of a row of dtype DT as floats
+template <int DT, int VB> struct Piece {
+  static constexpr int ES = DT == 1 ? 4 : 2, N = VB / ES;
+  using R = typename Raw<VB>::T;
+  static __device__ __forceinline__ R load(const void* p, int64_t byte) { return *(const R*)((const char*)p + byte); }
+  static __device__ __forceinline__ void unpack(const R& r, float (&x)[N]) {
+    if constexpr (VB == 2) {
+      x[0] = DT == 0 ? bf2f(r) : h2f(r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VB / 4; ++i) {
+        uint32_t w;
+        if constexpr (VB == 4) w = r;
+        else w = r[i];
+        if constexpr (DT == 1) x[i] = __builtin_bit_cast(float, w);
+        else if constexpr (DT == 0) {
+          x[2 * i] = __builtin_bit_cast(float, w << 16);
+          x[2 * i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
+        } else {
+          unpack_h2(w, x[2 * i], x[2 * i + 1]);
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ void store(void* p, int64_t byte, const float (&x)[N]) {
+    R r;
+    if constexpr (VB == 2) {
+      r = DT == 0 ? f2bf(x[0]) : f2h(x[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VB / 4; ++i) {
+        uint32_t w;
+        if constexpr (DT == 1) w = __builtin_bit_cast(uint32_t, x[i]);
+        else if constexpr (DT == 0) w = pack_bf2(x[2 * i], x[2 * i + 1]);
+        else w = pack_h2(x[2 * i], x[2 * i + 1]);
+        if constexpr (VB == 4) r = w;
+        else r[i] = w;
+      }
+    }
+    *(R*)((char*)p + byte) = r;
+  }
+};
 
 __device__ __forceinline__ int64_t load_id(const void* p, int bytes, int64_t i) {
   return bytes == 8 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
@@ -37,80 +83,441 @@ __device__ __forceinline__ float product(float x, float s) {
 
 }  // namespace
 
-template <int DT> __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a) {
-  const int64_t row = blockIdx.x;
-  const int64_t id = load_id(a.ids, a.id_bytes, row);
-  const bool ok = id >= 0 && id < a.V;
-  for (int j = threadIdx.x; j < a.H; j += 256)
-    put<DT>(a.y, row * a.y_rs + j, ok ? product(elem<DT>(a.x, id * a.x_rs + j), a.scale) : NAN);
+// ------------------------------------------------------------------ lookup
+constexpr int LOOKUP_ROWS = 4;  // rows a group of lanes has in flight
+
+template <int DT, int VB> __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a) {
+  using P = Piece<DT, VB>;
+  const int sub = threadIdx.x & (a.lpr - 1), grp = threadIdx.x / a.lpr, ng = 256 / a.lpr;
+  const int64_t t0 = ((int64_t)blockIdx.x * ng + grp) * LOOKUP_ROWS;
+  int64_t id[LOOKUP_ROWS];
+#pragma unroll
+  for (int i = 0; i < LOOKUP_ROWS; ++i) id[i] = t0 + i < a.n ? load_id(a.ids, a.id_bytes, t0 + i) : -1;
+  for (int c = sub; c < a.pieces; c += a.lpr) {
+    typename P::R r[LOOKUP_ROWS] = {};
+#pragma unroll
+    for (int i = 0; i < LOOKUP_ROWS; ++i)
+      if (id[i] >= 0 && id[i] < a.V) r[i] = P::load(a.x, id[i] * a.x_rs * P::ES + (int64_t)c * VB);
+#pragma unroll
+    for (int i = 0; i < LOOKUP_ROWS; ++i) {
+      if (t0 + i >= a.n) break;
+      float x[P::N];
+      P::unpack(r[i], x);
+#pragma unroll
+      for (int e = 0; e < P::N; ++e) x[e] = id[i] >= 0 && id[i] < a.V ? product(x[e], a.scale) : NAN;
+      P::store(a.y, (t0 + i) * a.y_rs * P::ES + (int64_t)c * VB, x);
+    }
+  }
 }
 
+// ------------------------------------------------------------------ sorting the tokens
 // The key of a token: its id, or V (behind every row of the vocabulary) when its gradient goes nowhere.
 __device__ __forceinline__ int32_t token_key(const EmbedArgs& a, int64_t t) {
   const int64_t id = load_id(a.ids, a.id_bytes, t);
   return id < 0 || id >= a.V || id == a.pad ? (int32_t)a.V : (int32_t)id;
 }
 
-// A token's place in the sorted order is the number of tokens with a smaller key, or the same key and an earlier
-// position.
-__global__ __launch_bounds__(256) void embed_rank_kernel(EmbedArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  __shared__ int32_t tile[256];
-  const int32_t key = t < a.n ? token_key(a, t) : 0;
-  int32_t rank = 0;
-  for (int64_t u0 = 0; u0 < a.n; u0 += 256) {
-    __syncthreads();
-    tile[threadIdx.x] = u0 + threadIdx.x < a.n ? token_key(a, u0 + threadIdx.x) : 0x7fffffff;
-    __syncthreads();
-    for (int i = 0; i < 256; ++i) rank += tile[i] < key || (tile[i] == key && u0 + i < t) ? 1 : 0;
-  }
-  if (t < a.n) {
-    a.key[rank] = key;
-    a.order[rank] = (int32_t)t;
-  }
+// no token of any id yet: thread i of `n`
+__device__ __forceinline__ void clear_runs(const EmbedArgs& a, int64_t i, int64_t n) {
+  for (; i < a.V; i += n) a.run[i] = int2{0, 0};
 }
 
-template <int DT> __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedArgs a) {
-  const int32_t v = blockIdx.x;
-  auto first = [&](int32_t key) {  // the first place with a key of at least `key`
-    int64_t lo = 0, hi = a.n;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (a.key[mid] < key) lo = mid + 1;
-      else hi = mid;
+__global__ __launch_bounds__(256) void embed_clear_kernel(EmbedArgs a) {
+  clear_runs(a, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
+// Up to RANK_MAX tokens, in one launch: a token's place is the number of tokens with a smaller key, or the same key and
+// an earlier position.  A wave holds RANK_KEYS keys, 64 a register, and compares a register with one token's key at a
+// time: one vector comparison and two scalar instructions for 64 pairs.  Tokens of earlier registers come first at
+// equal keys, which is a comparison with key + 1; the token's own register takes its equal lanes below it as well.
+constexpr int RANK_MAX = 16384, RANK_KEYS = 4096, RANK_WAVES = 8;
+
+__global__ __launch_bounds__(RANK_WAVES * 64) void embed_rank_kernel(EmbedArgs a, int per_wave) {
+  __shared__ int32_t keys[RANK_KEYS];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = (int)a.n;
+  const int t0 = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * RANK_WAVES + w) * per_wave);
+  clear_runs(a, (int64_t)blockIdx.x * (RANK_WAVES * 64) + threadIdx.x, (int64_t)gridDim.x * (RANK_WAVES * 64));
+  int32_t mine = 0x7fffffff;  // lane i: the key and the place of token t0 + i
+  if (lane < per_wave && t0 + lane < n) mine = token_key(a, t0 + lane);
+  int32_t place = 0;
+  for (int u0 = 0; u0 < n; u0 += RANK_KEYS) {
+    __syncthreads();
+    int32_t x[RANK_KEYS / (RANK_WAVES * 64)];  // every load ahead of the first store
+#pragma unroll
+    for (int i = 0; i < RANK_KEYS / (RANK_WAVES * 64); ++i) {
+      const int u = u0 + i * (RANK_WAVES * 64) + threadIdx.x;
+      x[i] = token_key(a, min(u, n - 1));
+      x[i] = u < n ? x[i] : 0x7fffffff;
     }
-    return lo;
-  };
-  const int64_t i0 = first(v), i1 = first(v + 1);
-  for (int j = threadIdx.x; j < a.H; j += 256) {
-    float s = 0.f;
-    for (int64_t i = i0; i < i1; ++i) s += elem<DT>(a.x, a.order[i] * a.x_rs + j);
-    put<DT>(a.y, v * a.y_rs + j, product(s, a.scale));
+#pragma unroll
+    for (int i = 0; i < RANK_KEYS / (RANK_WAVES * 64); ++i) keys[i * (RANK_WAVES * 64) + threadIdx.x] = x[i];
+    __syncthreads();
+    int32_t k[RANK_KEYS / 64];
+#pragma unroll
+    for (int j = 0; j < RANK_KEYS / 64; ++j) k[j] = keys[j * 64 + lane];
+    const int regs = min(RANK_KEYS, n - u0 + 63) / 64;
+    for (int i = 0; i < per_wave && t0 + i < n; ++i) {
+      const int t = t0 + i, own = (t >> 6) - (u0 >> 6);
+      const int32_t key = __builtin_amdgcn_readlane(mine, i);
+      int cnt = 0;
+#pragma unroll
+      for (int j = 0; j < RANK_KEYS / 64; ++j) {
+        if (j % 8 == 0 && j >= regs) break;
+        cnt += __popcll(__ballot(k[j] < key + (j < own ? 1 : 0)));
+      }
+      if (own >= 0 && own < RANK_KEYS / 64)
+        cnt += __popcll(__ballot(keys[own * 64 + lane] == key) & ((1ull << (t & 63)) - 1));
+      place += lane == i ? cnt : 0;
+    }
+  }
+  if (lane < per_wave && t0 + lane < n) {
+    a.key[place] = mine;
+    a.order[place] = t0 + lane;
   }
 }
 
-int launch_embed_fwd(int dtype, const EmbedArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)a.n), block(256);
-  if (dtype == 0) hipLaunchKernelGGL(embed_fwd_kernel<0>, grid, block, 0, s, a);
-  else if (dtype == 1) hipLaunchKernelGGL(embed_fwd_kernel<1>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(embed_fwd_kernel<2>, grid, block, 0, s, a);
-  return hipGetLastError() == hipSuccess ? 0 : -7;
+// More tokens: least significant digits first, `bits` of them a pass, tiles of 1024 tokens.  A pass counts each
+// tile's digits, turns the counts into each tile's place within its digit, and moves the tokens.
+constexpr int TILE = 1024, MAXBITS = 10;
+
+struct SortArgs {
+  const int32_t *key_in, *order_in;  // NULL in the first pass, which takes the tokens themselves
+  int32_t *key_out, *order_out;
+  int32_t *hist;                     // [tiles][bins], then each tile's offset within the bin
+  int32_t *total;                    // [bins]
+  int tiles, shift, bits;
+};
+
+__device__ __forceinline__ int32_t sort_key(const EmbedArgs& a, const SortArgs& s, int64_t i) {
+  return s.key_in ? s.key_in[i] : token_key(a, i);
 }
 
-int64_t embed_bwd_workspace(int64_t n, int64_t, int) { return 2 * ((n + 3) / 4 * 4) * 4 + 16; }
+__global__ __launch_bounds__(TILE) void embed_hist_kernel(EmbedArgs a, SortArgs s) {
+  __shared__ int32_t h[1 << MAXBITS];
+  const int bins = 1 << s.bits, t = threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * TILE + t;
+  if (!s.key_in) clear_runs(a, i, (int64_t)gridDim.x * TILE);
+  if (t < bins) h[t] = 0;
+  __syncthreads();
+  if (i < a.n) atomicAdd(&h[(sort_key(a, s, i) >> s.shift) & (bins - 1)], 1);
+  __syncthreads();
+  if (t < bins) s.hist[(int64_t)blockIdx.x * bins + t] = h[t];
+}
+
+// a workgroup takes 32 bins; its 32 rows of threads each take a run of tiles
+__global__ __launch_bounds__(1024) void embed_scan_kernel(SortArgs s) {
+  __shared__ int32_t part[32][33];
+  const int bins = 1 << s.bits, c = threadIdx.x & 31, j = threadIdx.x >> 5, b = blockIdx.x * 32 + c;
+  const int per = (s.tiles + 31) / 32, k0 = min(j * per, s.tiles), k1 = min(k0 + per, s.tiles);
+  int32_t sum = 0;
+  if (b < bins)
+    for (int k = k0; k < k1; ++k) sum += s.hist[(int64_t)k * bins + b];
+  part[j][c] = sum;
+  __syncthreads();
+  int32_t run = 0;
+  for (int i = 0; i < j; ++i) run += part[i][c];
+  if (b >= bins) return;
+  if (j == 31) s.total[b] = run + sum;
+  for (int k = k0; k < k1; ++k) {
+    const int32_t x = s.hist[(int64_t)k * bins + b];
+    s.hist[(int64_t)k * bins + b] = run;
+    run += x;
+  }
+}
+
+// The stable place of a token in its tile: in a wave, the lanes below with the same digit (found by one ballot per bit);
+// between waves, a count per wave and digit in LDS.
+__global__ __launch_bounds__(TILE) void embed_scatter_kernel(EmbedArgs a, SortArgs s) {
+  __shared__ uint16_t cnt[TILE / 64][1 << MAXBITS];
+  __shared__ int32_t base[1 << MAXBITS], wsum[TILE / 64];
+  const int bins = 1 << s.bits, t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int64_t i = (int64_t)blockIdx.x * TILE + t;
+  // where each digit begins: an exclusive sum of the totals over the bins, one bin a thread
+  const int32_t tot = t < bins ? s.total[t] : 0;
+  int32_t inc = tot;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int32_t x = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += x;
+  }
+  if (lane == 63) wsum[w] = inc;
+  for (int k = t; k < (TILE / 64) * (1 << MAXBITS) / 2; k += TILE) ((uint32_t*)cnt)[k] = 0;
+  __syncthreads();
+  int32_t before = 0;
+  for (int k = 0; k < w; ++k) before += wsum[k];
+  if (t < bins) base[t] = before + inc - tot + s.hist[(int64_t)blockIdx.x * bins + t];
+  const bool live = i < a.n;
+  const int32_t key = live ? sort_key(a, s, i) : 0;
+  const int d = (key >> s.shift) & (bins - 1);
+  uint64_t same = __ballot(live);
+  for (int bit = 0; bit < s.bits; ++bit) {
+    const uint64_t m = __ballot((d >> bit) & 1);
+    same &= (d >> bit) & 1 ? m : ~m;
+  }
+  const int below = __popcll(same & ((1ull << lane) - 1));
+  if (live && below == 0) cnt[w][d] = (uint16_t)__popcll(same);
+  __syncthreads();
+  if (t < bins) {
+    uint32_t run = 0;
+#pragma unroll
+    for (int k = 0; k < TILE / 64; ++k) {
+      const uint32_t x = cnt[k][t];
+      cnt[k][t] = (uint16_t)run;
+      run += x;
+    }
+  }
+  __syncthreads();
+  if (live) {
+    const int32_t place = base[d] + cnt[w][d] + below;
+    s.key_out[place] = key;
+    s.order_out[place] = s.order_in ? s.order_in[i] : (int32_t)i;
+  }
+}
+
+// ------------------------------------------------------------------ sums of rows
+// Rows first, first + 1, ... of a list, added in order with `U` loads in flight
+template <int DT, int VB, int U = 8, class F>
+__device__ __forceinline__ void add_rows(const void* x, int64_t col, int64_t first, int64_t end, F row, float (&s)[Piece<DT, VB>::N]) {
+  using P = Piece<DT, VB>;
+  int64_t i = first;
+  for (; i + U <= end; i += U) {
+    typename P::R r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = P::load(x, row(i + u) + col);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[P::N];
+      P::unpack(r[u], v);
+#pragma unroll
+      for (int e = 0; e < P::N; ++e) s[e] += v[e];
+    }
+  }
+  for (; i < end; ++i) {
+    float v[P::N];
+    P::unpack(P::load(x, row(i) + col), v);
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) s[e] += v[e];
+  }
+}
+
+// A chunk of a.chunk sorted tokens: notes where runs begin and end in it, and if all of it has one id adds up its
+// rows, the workgroup's groups of lanes taking a run of tokens each and their sums added in order.
+template <int DT, int VB> __global__ __launch_bounds__(256) void embed_chunk_kernel(EmbedArgs a) {
+  using P = Piece<DT, VB>;
+  const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;  // a row's slices side by side
+  const int64_t c0 = (int64_t)bx * a.chunk, c1 = c0 + a.chunk;
+  if (slice == 0) {
+    for (int64_t i = c0 + threadIdx.x; i < min(c1, a.n); i += 256) {
+      const int32_t key = a.key[i], prev = i ? a.key[i - 1] : -1, next = i + 1 < a.n ? a.key[i + 1] : -1;
+      if (key == (int32_t)a.V) break;
+      if (key != prev) a.run[key].x = (int32_t)i;
+      if (key != next) a.run[key].y = (int32_t)i + 1;
+    }
+  }
+  if (c1 > a.n) return;
+  const int32_t key = a.key[c0];
+  if (key == (int32_t)a.V || a.key[c1 - 1] != key) return;
+  const int sub = threadIdx.x & (a.lpr - 1), grp = threadIdx.x / a.lpr, ng = 256 / a.lpr;
+  const int c = slice * a.lpr + sub;
+  __shared__ float red[256 * P::N];
+  float s[P::N] = {};
+  const int64_t i0 = c0 + (int64_t)a.chunk * grp / ng, i1 = c0 + (int64_t)a.chunk * (grp + 1) / ng;
+  if (c < a.pieces)
+    add_rows<DT, VB, 16>(a.x, (int64_t)c * VB, i0, i1, [&](int64_t i) { return (int64_t)a.order[i] * a.x_rs * P::ES; }, s);
+#pragma unroll
+  for (int e = 0; e < P::N; ++e) red[threadIdx.x * P::N + e] = s[e];
+  __syncthreads();
+  if (grp == 0 && c < a.pieces) {
+    for (int g = 1; g < ng; ++g)
+#pragma unroll
+      for (int e = 0; e < P::N; ++e) s[e] += red[(g * a.lpr + sub) * P::N + e];
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) a.part[(int64_t)bx * a.H + (int64_t)c * P::N + e] = s[e];
+  }
+}
+
+constexpr int SHORT_RUN = 32;  // tokens that one group of lanes adds up alone
+constexpr int MAX_ROWS = 64;   // rows of the vocabulary a workgroup takes
+
+// Rows v = bx + j (int)(gridDim.x / a.slices): frequent ids are neighbours, and so are shared out.  Each group of lanes takes the
+// workgroup's rows with short runs in turn; then the workgroup adds up each long run together, as the tokens ahead of
+// its first whole chunk, the chunks' sums, and the tokens behind the last, cut into as many equal parts as there
+// are groups, whose sums are added in order.
+template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedArgs a) {
+  using P = Piece<DT, VB>;
+  const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;
+  __shared__ int2 run[MAX_ROWS];
+  __shared__ float red[256 * P::N];
+  const int G = (int)(gridDim.x / a.slices), nr = (int)((a.V - bx + G - 1) / G);
+  if (threadIdx.x < nr) run[threadIdx.x] = a.run[bx + threadIdx.x * (int64_t)G];
+  __syncthreads();
+  const int sub = threadIdx.x & (a.lpr - 1), grp = threadIdx.x / a.lpr, ng = 256 / a.lpr;
+  const int c = slice * a.lpr + sub;
+  const int64_t col = (int64_t)c * VB;
+  auto token = [&](int64_t i) { return (int64_t)a.order[i] * a.x_rs * P::ES; };
+  auto put = [&](int j, float (&s)[P::N]) {
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) s[e] = product(s[e], a.scale);
+    P::store(a.y, (bx + j * (int64_t)G) * a.y_rs * P::ES + col, s);
+  };
+  if (c < a.pieces) {
+    for (int j = grp; j < nr; j += ng) {
+      const int32_t i0 = run[j].x, i1 = run[j].y;
+      if (i1 - i0 > SHORT_RUN) continue;
+      float s[P::N] = {};
+      add_rows<DT, VB>(a.x, col, i0, i1, token, s);
+      put(j, s);
+    }
+  }
+  for (int j = 0; j < nr; ++j) {
+    const int32_t i0 = run[j].x, i1 = run[j].y;
+    if (i1 - i0 <= SHORT_RUN) continue;
+    // items: [0, h) tokens i0.., [h, h + m) chunks k0.., [h + m, total) tokens behind the last chunk
+    const int32_t k0 = (i0 + a.chunk - 1) / a.chunk, k1 = i1 / a.chunk;
+    const bool chunks = k1 > k0;
+    const int32_t h = chunks ? k0 * a.chunk - i0 : i1 - i0, m = chunks ? k1 - k0 : 0;
+    const int32_t total = chunks ? h + m + (i1 - k1 * a.chunk) : h;
+    const int32_t b0 = (int32_t)((int64_t)total * grp / ng), b1 = (int32_t)((int64_t)total * (grp + 1) / ng);
+    float s[P::N] = {};
+    if (c < a.pieces) {
+      add_rows<DT, VB>(a.x, col, i0 + min(b0, h), i0 + min(b1, h), token, s);
+      for (int32_t k = k0 + min(max(b0 - h, 0), m); k < k0 + min(max(b1 - h, 0), m); ++k)
+#pragma unroll
+        for (int e = 0; e < P::N; ++e) s[e] += a.part[(int64_t)k * a.H + (int64_t)c * P::N + e];
+      const int64_t q = (int64_t)k1 * a.chunk - h - m;  // item b behind the chunks is token q + b
+      if (chunks) add_rows<DT, VB>(a.x, col, q + max(b0, h + m), q + max(b1, h + m), token, s);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) red[threadIdx.x * P::N + e] = s[e];
+    __syncthreads();
+    if (grp == 0 && c < a.pieces) {
+      for (int g = 1; g < ng; ++g)
+#pragma unroll
+        for (int e = 0; e < P::N; ++e) s[e] += red[(g * a.lpr + sub) * P::N + e];
+      put(j, s);
+    }
+  }
+}
+
+namespace {
+
+// the bytes a lane takes of a row: the most that the row's length, its strides and its addresses are multiples of
+int piece_bytes(int es, const EmbedArgs& a) {
+  const uint64_t all = (uint64_t)(uintptr_t)a.x | (uintptr_t)a.y | (uint64_t)(a.x_rs * es) | (uint64_t)(a.y_rs * es) |
+                       (uint64_t)((int64_t)a.H * es);
+  for (int vb = 16; vb > es; vb /= 2)
+    if (all % vb == 0) return vb;
+  return es;
+}
+
+template <class F> int with_piece(int dtype, int vb, F&& f) {
+  using std::integral_constant;
+  auto go = [&](auto dt, auto v) { return f(dt, v); };
+#define PE_PIECE(D, B) \
+  if (dtype == D && vb == B) return go(integral_constant<int, D>{}, integral_constant<int, B>{})
+  PE_PIECE(0, 16); PE_PIECE(0, 8); PE_PIECE(0, 4); PE_PIECE(0, 2);
+  PE_PIECE(1, 16); PE_PIECE(1, 8); PE_PIECE(1, 4);
+  PE_PIECE(2, 16); PE_PIECE(2, 8); PE_PIECE(2, 4); PE_PIECE(2, 2);
+#undef PE_PIECE
+  return -4;
+}
+
+// lanes a row: the power of two that covers its pieces, from 8 up to `most`
+int lanes_per_row(int pieces, int most) {
+  int l = 8;
+  while (l < most && l < pieces) l *= 2;
+  return l;
+}
+
+int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
+
+// sorted tokens a chunk: at most 8192 chunks, so that their sums stay small beside the gradient
+int chunk_tokens(int64_t n) {
+  int c = 64;
+  while (n / c > 8192) c *= 2;
+  return c;
+}
+
+int key_bits(int64_t V) {  // of keys 0 .. V
+  int b = 1;
+  while ((int64_t)1 << b <= V) ++b;
+  return b;
+}
+
+int done() { return hipGetLastError() == hipSuccess ? 0 : -7; }
+
+}  // namespace
+
+int launch_embed_fwd(int dtype, EmbedArgs a, hipStream_t s) {
+  const int es = dtype == 1 ? 4 : 2, vb = piece_bytes(es, a);
+  a.pieces = (int)((int64_t)a.H * es / vb);
+  a.lpr = lanes_per_row(a.pieces, 256);
+  const int64_t rows = (int64_t)(256 / a.lpr) * LOOKUP_ROWS;
+  const dim3 grid((unsigned)((a.n + rows - 1) / rows)), block(256);
+  return with_piece(dtype, vb, [&](auto dt, auto v) {
+    hipLaunchKernelGGL((embed_fwd_kernel<decltype(dt)::value, decltype(v)::value>), grid, block, 0, s, a);
+    return done();
+  });
+}
+
+// each id's run; [key][order] of the sorted tokens; past RANK_MAX tokens a second pair and the counts; the chunks' sums
+int64_t embed_bwd_workspace(int64_t n, int64_t V, int H) {
+  int64_t w = up4(2 * V) + 2 * up4(n);
+  if (n > RANK_MAX) w += 2 * up4(n) + ((n + TILE - 1) / TILE + 1) * (1 << MAXBITS);
+  return 4 * (w + n / chunk_tokens(n) * (int64_t)H) + 16;
+}
 
 int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s) {
-  a.key = (int32_t*)ws;
-  a.order = a.key + (a.n + 3) / 4 * 4;
-  if (a.n) {
-    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((a.n + 255) / 256)), dim3(256), 0, s, a);
-    if (hipGetLastError() != hipSuccess) return -7;
+  const int es = dtype == 1 ? 4 : 2, vb = piece_bytes(es, a);
+  int32_t* p = (int32_t*)ws;
+  auto take = [&](int64_t n) { int32_t* q = p; p += n; return q; };
+  a.run = (int2*)take(up4(2 * a.V));
+  a.key = take(up4(a.n));
+  a.order = take(up4(a.n));
+  if (a.n > RANK_MAX) {
+    int32_t *key2 = take(up4(a.n)), *order2 = take(up4(a.n));
+    SortArgs o;
+    o.tiles = (int)((a.n + TILE - 1) / TILE);
+    o.hist = take((int64_t)o.tiles << MAXBITS);
+    o.total = take(1 << MAXBITS);
+    const int bits = key_bits(a.V), passes = (bits + MAXBITS - 1) / MAXBITS;
+    o.bits = (bits + passes - 1) / passes;
+    for (int i = 0; i < passes; ++i) {
+      const bool last_in_first = (passes - 1 - i) % 2 == 0;  // the last pass writes a.key / a.order
+      o.key_in = i == 0 ? nullptr : (last_in_first ? key2 : a.key);
+      o.order_in = i == 0 ? nullptr : (last_in_first ? order2 : a.order);
+      o.key_out = last_in_first ? a.key : key2;
+      o.order_out = last_in_first ? a.order : order2;
+      o.shift = i * o.bits;
+      hipLaunchKernelGGL(embed_hist_kernel, dim3(o.tiles), dim3(TILE), 0, s, a, o);
+      hipLaunchKernelGGL(embed_scan_kernel, dim3(((1 << o.bits) + 31) / 32), dim3(1024), 0, s, o);
+      hipLaunchKernelGGL(embed_scatter_kernel, dim3(o.tiles), dim3(TILE), 0, s, a, o);
+    }
+  } else if (a.n) {
+    // about one workgroup per compute unit
+    const int per_wave = std::max(1, (int)((a.n + 256 * RANK_WAVES - 1) / (256 * RANK_WAVES)));
+    const int64_t per = (int64_t)per_wave * RANK_WAVES;
+    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((a.n + per - 1) / per)), dim3(RANK_WAVES * 64), 0, s, a, per_wave);
+  } else {
+    hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)((a.V + 255) / 256)), dim3(256), 0, s, a);
   }
-  const dim3 grid((unsigned)a.V), block(256);
-  if (dtype == 0) hipLaunchKernelGGL(embed_bwd_kernel<0>, grid, block, 0, s, a);
-  else if (dtype == 1) hipLaunchKernelGGL(embed_bwd_kernel<1>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(embed_bwd_kernel<2>, grid, block, 0, s, a);
-  return hipGetLastError() == hipSuccess ? 0 : -7;
+  if (hipGetLastError() != hipSuccess) return -7;
+  a.part = (float*)p;
+  a.chunk = chunk_tokens(a.n);
+  a.pieces = (int)((int64_t)a.H * es / vb);
+  a.lpr = lanes_per_row(a.pieces, 64);
+  a.slices = (a.pieces + a.lpr - 1) / a.lpr;
+  const unsigned chunks = (unsigned)((a.n + a.chunk - 1) / a.chunk);
+  const unsigned rows = (unsigned)((a.V + MAX_ROWS - 1) / MAX_ROWS);
+  const unsigned grid = (unsigned)std::min<int64_t>(a.V, std::max<int64_t>(rows, 1024));
+  if ((int64_t)std::max(grid, chunks) * a.slices > 0x7fffffff) return -2;
+  return with_piece(dtype, vb, [&](auto dt, auto v) {
+    constexpr int D = decltype(dt)::value, B = decltype(v)::value;
+    if (chunks) hipLaunchKernelGGL((embed_chunk_kernel<D, B>), dim3(chunks * a.slices), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((embed_bwd_kernel<D, B>), dim3(grid * a.slices), dim3(256), 0, s, a);
+    return done();
+  });
 }
 
 }  // namespace pe

@@ -323,8 +323,11 @@ struct EmbedArgs {
   void* y; int64_t y_rs;        // the looked-up rows, or the gradient of the weight
   int64_t V; int H; float scale; int64_t pad;
   int32_t *key, *order;         // the tokens sorted by id: their ids and positions
+  int2* run;                    // each id's first sorted token and the one behind its last
+  float* part; int chunk;       // sums over chunks of sorted tokens
+  int pieces, lpr, slices;      // vector accesses a row, lanes that work on one, and its column slices
 };
-int launch_embed_fwd(int dtype, const EmbedArgs& a, hipStream_t s);
+int launch_embed_fwd(int dtype, EmbedArgs a, hipStream_t s);
 int64_t embed_bwd_workspace(int64_t n, int64_t V, int H);
 int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s);
 

@@ -48,7 +48,7 @@ def test_training_step(cuda, tie):
     assert torch.equal(ref, out["logits"])
     loss = plain_loss(ref, labels)
     loss.backward()
-    assert abs(float(loss) - float(out["loss"])) < 1e-5
+    assert abs(float(loss.detach()) - float(out["loss"].detach())) < 1e-5
     for n, p in m.named_parameters():
         # fp32 gradients through the same kernels: the two paths differ by roundings of their sums
         assert (p.grad - got[n]).norm() <= 1e-4 * p.grad.norm() + 1e-9, n
