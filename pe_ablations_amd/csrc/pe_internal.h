@@ -304,13 +304,14 @@ struct LossArgs {
   const void* tlog; int64_t tlog_rs; int tlog_dtype;
   int64_t rows; int V, K, reduction;
   float hw, sw, T, factor;
+  int stream;             // store the gradient past the caches
   float* row_loss;        // one per row
   float* stats;           // [rows][3]: maximum, sum, sum at the temperature; [3 rows]: 1 / rows that count
   const float* dloss;     // one, or one per row (PE_LOSS_NONE)
   const float* inv_count; // 1 / rows that count (PE_LOSS_MEAN)
 };
 enum { LOSS_FWD = 0, LOSS_BWD = 1, LOSS_STEP = 2 };
-int launch_loss(int dtype, int phase, const LossArgs& a, hipStream_t s);
+int launch_loss(int dtype, int phase, LossArgs a, hipStream_t s);
 // 1 / rows that count (PE_LOSS_MEAN) from the labels
 int launch_loss_count(const LossArgs& a, float* inv_count, hipStream_t s);
 // the sum or mean of row_loss; also 1 / rows that count when inv_count is not NULL

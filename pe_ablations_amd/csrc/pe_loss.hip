@@ -36,16 +36,22 @@ __device__ __forceinline__ int64_t load_id(const void* p, int bytes, int64_t i) 
 }
 
 // the row's label; false when the row does not count.  Without labels every row counts, with label -1
-__device__ __forceinline__ bool row_label(const LossArgs& a, int64_t r, int64_t& y) {
+__device__ __forceinline__ bool row_label(const LossArgs& a, uint32_t r, int64_t& y) {
   y = -1;
   if (!a.labels) return true;
   if (a.shift) {
-    if (r % a.shift == a.shift - 1) return false;
     r += 1;
+    if (r % (uint32_t)a.shift == 0) return false;
   }
   y = load_id(a.labels, a.label_bytes, r);
   return y != a.ignore;
 }
+
+// What is summed.  At temperature 1 both parts have the same exponentials, at 2 the hard part's are the squares of
+// the soft part's: one exponential an element in place of two.
+enum { HARD = 1, SOFT = 2, BOTH = 3, BOTH_T1 = 4, BOTH_T2 = 5 };
+constexpr bool has_hard(int mode) { return mode != SOFT; }
+constexpr bool has_soft(int mode) { return mode != HARD; }
 
 // 2^x in one instruction; results below 2^-126 are 0
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -90,12 +96,20 @@ template <int DT> struct Row {
     return j < V ? j : -1;
   }
   __device__ __forceinline__ int first(int k) const { return head + k * Vec<DT>::N; }  // element of piece k
-  __device__ __forceinline__ u32x4 load(int k) const { return *(const u32x4*)(p + (int64_t)first(k) * Vec<DT>::ES); }
+  template <bool NT> __device__ __forceinline__ u32x4 load(int k) const {
+    const u32x4* q = (const u32x4*)(p + (int64_t)first(k) * Vec<DT>::ES);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+  }
 };
 // the pieces of a row whose gradient is 16 bytes aligned where the row is, else element by element
-template <int DT> __device__ __forceinline__ void store_piece(char* dz, int j, bool together, const float (&x)[Vec<DT>::N]) {
-  if (together) {
-    *(u32x4*)(dz + (int64_t)j * Vec<DT>::ES) = Vec<DT>::pack(x);
+enum { STORE_ELEMENTS, STORE_PLAIN, STORE_STREAM };
+template <int DT> __device__ __forceinline__ void store_piece(char* dz, int j, int how, const float (&x)[Vec<DT>::N]) {
+  u32x4* q = (u32x4*)(dz + (int64_t)j * Vec<DT>::ES);
+  if (how == STORE_STREAM) {
+    __builtin_nontemporal_store(Vec<DT>::pack(x), q);
+    asm volatile("");  // else the compiler makes one plain store of the two
+  } else if (how == STORE_PLAIN) {
+    *q = Vec<DT>::pack(x);
   } else {
 #pragma unroll
     for (int e = 0; e < Vec<DT>::N; ++e) put<DT>(dz, j + e, x[e]);
@@ -107,80 +121,174 @@ template <int DT> __device__ __forceinline__ void store_piece(char* dz, int j, b
 struct Stat { float m, s, t; };
 __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 
-template <bool HARD, bool SOFT> __device__ __forceinline__ void rescale(Stat& x, float m, float lt) {
-  const float d = x.m - reference(m);
-  if (HARD) x.s *= ex2(d * LOG2E);
-  if (SOFT) x.t *= ex2(d * lt);
+// the exponentials of an element d above (below 0) the maximum: of the hard part, and of the soft part
+template <int MODE> __device__ __forceinline__ void exps(float d, float lt, float& e, float& et) {
+  e = et = 0.f;
+  if (MODE == BOTH_T2) {
+    et = ex2(d * (0.5f * LOG2E));
+    e = et * et;
+  } else {
+    if (has_hard(MODE)) e = ex2(d * LOG2E);
+    if (MODE == SOFT || MODE == BOTH) et = ex2(d * lt);
+  }
+  if (MODE == BOTH_T1) et = e;
+}
+template <int MODE> __device__ __forceinline__ void rescale(Stat& x, float m, float lt) {
+  float e, et;
+  exps<MODE>(x.m - reference(m), lt, e, et);
+  if (has_hard(MODE)) x.s *= e;
+  if (has_soft(MODE)) x.t *= et;
   x.m = m;
 }
-template <bool HARD, bool SOFT, int N> __device__ __forceinline__ void add(Stat& st, const float (&x)[N], float lt) {
+template <int MODE, int N> __device__ __forceinline__ void add(Stat& st, const float (&x)[N], float lt) {
   const float ref = reference(st.m);
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float d = x[e] - ref;
-    if (HARD) st.s += ex2(d * LOG2E);
-    if (SOFT) st.t += ex2(d * lt);
+  for (int i = 0; i < N; ++i) {
+    float e, et;
+    exps<MODE>(x[i] - ref, lt, e, et);
+    if (has_hard(MODE)) st.s += e;
+    if (has_soft(MODE)) st.t += et;
   }
 }
-template <bool HARD, bool SOFT> __device__ __forceinline__ Stat join(Stat x, Stat y, float lt) {
+template <int MODE> __device__ __forceinline__ Stat join(Stat x, Stat y, float lt) {
   const float m = fmaxf(x.m, y.m);
-  rescale<HARD, SOFT>(x, m, lt);
-  rescale<HARD, SOFT>(y, m, lt);
+  rescale<MODE>(x, m, lt);
+  rescale<MODE>(y, m, lt);
   return Stat{m, x.s + y.s, x.t + y.t};
 }
 
-template <int T> __device__ __forceinline__ float block_sum(float v, float* red) {
+__device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  __syncthreads();
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+template <int T> __device__ __forceinline__ float block_sum(float v, float* red) {
+  v = wave_sum(v);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   float r = red[0];
+#pragma unroll
   for (int i = 1; i < T / 64; ++i) r += red[i];
   return r;
 }
 template <int T> __device__ __forceinline__ float block_max(float v, float* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  __syncthreads();
+  v = wave_max(v);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   float r = red[0];
+#pragma unroll
   for (int i = 1; i < T / 64; ++i) r = fmaxf(r, red[i]);
   return r;
 }
 
 }  // namespace
 
-constexpr int U = 4;  // pieces a thread has in flight where the row is not held
+// The teacher's pairs of a row, by one wave: the places whose gradient is more than the dense one, that is every
+// different id among the pairs present, with the sum of its probabilities, and the label if it is none of them (y < 0:
+// no label), into `place` / `prob` [K + 1] (-1 where there is none); whether any pair is present, P, and
+// E = sum p ln p.  `tid` and `tp` [K] are the pairs themselves (-1 where absent), which do for the loss (MERGE false).
+template <bool MERGE>
+__device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, float lt, int32_t y, int32_t* tid, float* tp,
+                                            int32_t* place, float* prob, float& P, float& E) {
+  const int lane = threadIdx.x & 63;
+  float mx = -INFINITY;
+  for (int k = lane; k < a.K; k += 64) {
+    const int64_t id = load_id(a.tid, a.tid_bytes, r * a.tid_rs + k);
+    const float x = load_as_float(a.tlog, r * a.tlog_rs + k, a.tlog_dtype);
+    const bool have = id >= 0 && id < a.V && x != -INFINITY;
+    tid[k] = have ? (int32_t)id : -1;
+    tp[k] = x;
+    if (have) mx = fmaxf(mx, x);
+  }
+  mx = wave_max(mx);
+  float n = 0.f;
+  for (int k = lane; k < a.K; k += 64)
+    if (tid[k] >= 0) n += ex2((tp[k] - mx) * lt);
+  n = wave_sum(n);
+  P = n != 0.f ? 1.f : 0.f;
+  const float ln = logf(n);
+  E = 0.f;
+  for (int k = lane; k < a.K; k += 64) {
+    float p = 0.f;
+    if (tid[k] >= 0) {
+      const float d = tp[k] - mx;
+      p = ex2(d * lt) / n;
+      if (p != 0.f) E += p * (d / a.T - ln);
+    }
+    tp[k] = p;
+  }
+  E = wave_sum(E);
+  if (!MERGE) return;
+  bool label = false;  // among the pairs
+  for (int k = lane; k < a.K; k += 64) {
+    const int32_t id = tid[k];
+    float p = 0.f;
+    bool first = id >= 0;
+#pragma unroll 4
+    for (int i = 0; i < a.K; ++i) {
+      const bool same = tid[i] == id;
+      first = first && !(same && i < k);
+      p += same ? tp[i] : 0.f;
+    }
+    place[k] = first ? id : -1;
+    prob[k] = p;
+    label = label || id == y;
+  }
+  label = __ballot(label) != 0;
+  if (lane == 0) {
+    place[a.K] = label ? -1 : y;
+    prob[a.K] = 0.f;
+  }
+}
+
+// gradients beyond this size are stored past the 256 MB cache
+#ifndef STREAMB
+#define STREAMB (128ll << 20)
+#endif
+constexpr int64_t STREAM_BYTES = STREAMB;
+
+constexpr int LOSS_ALONE = 3;  // a forward without a backward to follow: the logits are read past the caches
 
 // NC > 0: the row is held in registers, NC pieces a thread (the step, rows of up to NC T pieces); 0: it is read
-// once for the sums (forward) or the gradient (backward), or for both in turn (the step of a longer row)
-template <int DT, int PHASE, bool HARD, bool SOFT, int T, int NC>
+// once for the sums (forward) or the gradient (backward), or for both in turn (the step of a longer row), U pieces a
+// thread in flight.
+//
+// The backward takes the rows last to first: those that the forward read last are still in the 256 MB cache behind
+// the L2s, and a gradient that does not fit there is stored past it (4096 x 50257 in bf16, forward and backward:
+// 244 us, 233 us with such stores, 214 us in reverse as well).
+template <int DT, int PHASE, int MODE, int T, int NC, int U>
 __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
-  __shared__ float red[T / 64];
+  constexpr bool FWD = PHASE == LOSS_FWD || PHASE == LOSS_ALONE, BWD = PHASE == LOSS_BWD, NT = PHASE == LOSS_ALONE;
+  __shared__ float red[2][T / 64];
   __shared__ Stat wred[T / 64];
-  __shared__ int32_t tid_l[SOFT ? PE_LOSS_MAX_TOP_K : 1];  // the teacher's ids, -1 where absent
-  __shared__ float tp_l[SOFT ? PE_LOSS_MAX_TOP_K : 1];     // and probabilities
+  constexpr int KMAX = has_soft(MODE) ? PE_LOSS_MAX_TOP_K + 1 : 1;
+  __shared__ float tsum[2];  // teacher_row's P and E, and its arrays
+  __shared__ int32_t tid_l[KMAX], place[FWD ? 1 : KMAX];
+  __shared__ float tp_l[KMAX], prob[FWD ? 1 : KMAX];
   using W = Vec<DT>;
   constexpr int N = W::N;
-  const int64_t r = blockIdx.x;
+  const int64_t r = BWD ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
   const int t = threadIdx.x, V = a.V;
   const char* z = (const char*)a.z + r * a.z_rs * W::ES;
-  char* dz = PHASE == LOSS_FWD ? nullptr : (char*)a.dz + r * a.dz_rs * W::ES;
+  char* dz = FWD ? nullptr : (char*)a.dz + r * a.dz_rs * W::ES;
   const Row<DT> row(z, V);
   const int one = row.single(t);
-  const bool together = (((uintptr_t)z ^ (uintptr_t)dz) & 15) == 0;
+  const int how = ((uintptr_t)z ^ (uintptr_t)dz) & 15 ? STORE_ELEMENTS : (a.stream ? STORE_STREAM : STORE_PLAIN);
   int64_t y;
-  if (!row_label(a, r, y)) {
-    if (PHASE != LOSS_FWD) {
+  if (!row_label(a, (uint32_t)r, y)) {
+    if (!FWD) {
       const float zero[N] = {};
-      for (int k = t; k < row.nvec; k += T) store_piece<DT>(dz, row.first(k), together, zero);
+      for (int k = t; k < row.nvec; k += T) store_piece<DT>(dz, row.first(k), how, zero);
       if (one >= 0) put<DT>(dz, one, 0.f);
     }
     if (t == 0) {
-      if (PHASE != LOSS_BWD) a.row_loss[r] = 0.f;
-      if (PHASE == LOSS_FWD && a.stats) a.stats[3 * r] = a.stats[3 * r + 1] = a.stats[3 * r + 2] = 0.f;
+      if (!BWD) a.row_loss[r] = 0.f;
+      if (PHASE == LOSS_FWD) a.stats[3 * r] = a.stats[3 * r + 1] = a.stats[3 * r + 2] = 0.f;
     }
     return;
   }
@@ -189,13 +297,23 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
 
   Stat st{-INFINITY, 0.f, 0.f};
   u32x4 held[NC > 0 ? NC : 1];
-  const float xone = one >= 0 ? elem<DT>(z, one) : -INFINITY;
-  if (PHASE == LOSS_BWD) {
-    st = Stat{a.stats[3 * r], a.stats[3 * r + 1], a.stats[3 * r + 2]};
-  } else if (NC > 0) {
+  if (NC > 0) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-      if (c * T + t < row.nvec) held[c] = row.load(c * T + t);
+      if (c * T + t < row.nvec) held[c] = row.template load<false>(c * T + t);
+  }
+  const float xone = one >= 0 ? elem<DT>(z, one) : -INFINITY;
+  if (has_soft(MODE) && t >= T - 64) {  // the last wave, which has the fewest pieces; the others need it behind a barrier only
+    float P, E;
+    teacher_row<!FWD>(a, r, lt, has_hard(MODE) && !bad ? (int32_t)y : -1, tid_l, tp_l, place, prob, P, E);
+    if (t == T - 64) {
+      tsum[0] = P;
+      tsum[1] = E;
+    }
+  }
+  if (BWD) {
+    st = Stat{a.stats[3 * r], a.stats[3 * r + 1], a.stats[3 * r + 2]};
+  } else if (NC > 0) {
     float mx = xone;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -206,28 +324,30 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
         for (int e = 0; e < N; ++e) mx = fmaxf(mx, x[e]);
       }
     }
-    st.m = block_max<T>(mx, red);
+    st.m = block_max<T>(mx, red[0]);
     const float x1[1] = {xone};
-    add<HARD, SOFT>(st, x1, lt);
+    add<MODE>(st, x1, lt);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if (c * T + t < row.nvec) {
         float x[N];
         W::unpack(held[c], x);
-        add<HARD, SOFT>(st, x, lt);
+        add<MODE>(st, x, lt);
       }
     }
-    if (HARD) st.s = block_sum<T>(st.s, red);
-    if (SOFT) st.t = block_sum<T>(st.t, red);
+    if (has_hard(MODE)) st.s = block_sum<T>(st.s, red[1]);
+    if (MODE == SOFT) st.t = block_sum<T>(st.t, red[1]);
+    else if (MODE == BOTH_T1) st.t = st.s;
+    else if (has_soft(MODE)) st.t = block_sum<T>(st.t, (float*)wred);
   } else {
     const float x1[1] = {xone};
     st.m = xone;
-    add<HARD, SOFT>(st, x1, lt);
+    add<MODE>(st, x1, lt);
     int k = t;
     for (; k + (U - 1) * T < row.nvec; k += U * T) {
       u32x4 raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = row.load(k + u * T);
+      for (int u = 0; u < U; ++u) raw[u] = row.template load<NT>(k + u * T);
       float x[U][N], mx = st.m;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -235,94 +355,71 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
 #pragma unroll
         for (int e = 0; e < N; ++e) mx = fmaxf(mx, x[u][e]);
       }
-      rescale<HARD, SOFT>(st, mx, lt);
+      rescale<MODE>(st, mx, lt);
 #pragma unroll
-      for (int u = 0; u < U; ++u) add<HARD, SOFT>(st, x[u], lt);
+      for (int u = 0; u < U; ++u) add<MODE>(st, x[u], lt);
     }
     for (; k < row.nvec; k += T) {
       float x[N], mx = st.m;
-      W::unpack(row.load(k), x);
+      W::unpack(row.template load<NT>(k), x);
 #pragma unroll
       for (int e = 0; e < N; ++e) mx = fmaxf(mx, x[e]);
-      rescale<HARD, SOFT>(st, mx, lt);
-      add<HARD, SOFT>(st, x, lt);
+      rescale<MODE>(st, mx, lt);
+      add<MODE>(st, x, lt);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
-      st = join<HARD, SOFT>(st, Stat{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)}, lt);
+      st = join<MODE>(st, Stat{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)}, lt);
     if ((t & 63) == 0) wred[t >> 6] = st;
     __syncthreads();
     st = wred[0];
-    for (int i = 1; i < T / 64; ++i) st = join<HARD, SOFT>(st, wred[i], lt);
+    for (int i = 1; i < T / 64; ++i) st = join<MODE>(st, wred[i], lt);
   }
-  if (PHASE == LOSS_FWD && a.stats && t == 0) {
-    a.stats[3 * r] = st.m;
-    a.stats[3 * r + 1] = st.s;
-    a.stats[3 * r + 2] = st.t;
-  }
-
-  // the teacher's probabilities
-  float P = 0.f;
-  if (SOFT) {
-    float mx = -INFINITY;
-    for (int k = t; k < a.K; k += T) {
-      const int64_t id = load_id(a.tid, a.tid_bytes, r * a.tid_rs + k);
-      const float x = load_as_float(a.tlog, r * a.tlog_rs + k, a.tlog_dtype);
-      const bool have = id >= 0 && id < V && x != -INFINITY;
-      tid_l[k] = have ? (int32_t)id : -1;
-      tp_l[k] = x;
-      if (have) mx = fmaxf(mx, x);
+  // without a pair the soft part is 0, which an infinite sum makes of its gradient
+  if (!BWD && has_soft(MODE) && tsum[0] == 0.f) st.t = INFINITY;
+  if (!BWD && t < 64) {  // the first wave: the row's loss
+    float cross = 0.f;   // sum p (m - z) / T
+    if (has_soft(MODE)) {
+      for (int k = t; k < a.K; k += 64)
+        if (tp_l[k] != 0.f) cross += tp_l[k] * (st.m - elem<DT>(z, tid_l[k]));
+      cross = wave_sum(cross) / a.T;
     }
-    mx = block_max<T>(mx, red);
-    float n = 0.f;
-    for (int k = t; k < a.K; k += T)
-      if (tid_l[k] >= 0) n += ex2((tp_l[k] - mx) * lt);
-    n = block_sum<T>(n, red);
-    P = n != 0.f ? 1.f : 0.f;
-    float sum = 0.f;
-    for (int k = t; k < a.K; k += T) {
-      float p = 0.f;
-      if (tid_l[k] >= 0) {
-        const float d = tp_l[k] - mx;
-        p = ex2(d * lt) / n;
-        if (PHASE != LOSS_BWD && p != 0.f)
-          sum += p * ((d + st.m - elem<DT>(z, tid_l[k])) / a.T - logf(n) + logf(st.t));
-      }
-      tp_l[k] = p;
-    }
-    if (PHASE != LOSS_BWD) {
-      sum = block_sum<T>(sum, red);
-      P = n != 0.f ? 1.f : 0.f;
-      if (t == 0) {
-        float loss = a.sw * a.T * a.T * sum;
-        if (HARD) loss += a.hw * (bad ? NAN : (st.m - elem<DT>(z, y)) + logf(st.s));
-        a.row_loss[r] = bad ? NAN : loss;
+    if (t == 0) {
+      float loss = 0.f;
+      if (has_soft(MODE) && tsum[0] != 0.f) loss = a.sw * a.T * a.T * (tsum[1] + cross + logf(st.t));
+      if (has_hard(MODE) && !bad) loss += a.hw * ((st.m - elem<DT>(z, y)) + logf(st.s));
+      a.row_loss[r] = bad ? NAN : loss;
+      if (PHASE == LOSS_FWD) {
+        a.stats[3 * r] = st.m;
+        a.stats[3 * r + 1] = st.s;
+        a.stats[3 * r + 2] = st.t;
       }
     }
-    __syncthreads();
-  } else if (PHASE != LOSS_BWD && t == 0) {
-    a.row_loss[r] = bad ? NAN : a.hw * ((st.m - elem<DT>(z, y)) + logf(st.s));
   }
+  if (FWD) return;
 
-  if (PHASE == LOSS_FWD) return;
   float c = a.factor;
   if (a.dloss) c *= a.dloss[a.reduction == PE_LOSS_NONE ? r : 0];
   if (a.inv_count) c *= *a.inv_count;
   if (bad) c = NAN;
-  const float ch = HARD ? c * a.hw / st.s : 0.f, ct = SOFT ? c * a.sw * a.T * P / st.t : 0.f;
+  float ch = 0.f, ct = 0.f;
+  if (has_hard(MODE)) ch = c * a.hw / st.s;
+  if (has_soft(MODE)) ct = c * a.sw * a.T / st.t;
   auto dense = [&](float x) {
-    const float d = x - st.m;
-    float g = 0.f;
-    if (HARD) g = ch * ex2(d * LOG2E);
-    if (SOFT) g = HARD ? g + ct * ex2(d * lt) : ct * ex2(d * lt);
-    return g;
+    float e, et;
+    exps<MODE>(x - st.m, lt, e, et);
+    if (MODE == HARD) return ch * e;
+    if (MODE == SOFT) return ct * et;
+    if (MODE == BOTH_T1) return (ch + ct) * e;
+    if (MODE == BOTH_T2) return et * (ch * et + ct);
+    return ch * e + ct * et;
   };
   auto piece = [&](int k, const u32x4& raw) {
     float x[N];
     W::unpack(raw, x);
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = dense(x[e]);
-    store_piece<DT>(dz, row.first(k), together, x);
+    store_piece<DT>(dz, row.first(k), how, x);
   };
   if (one >= 0) put<DT>(dz, one, dense(xone));
   if (NC > 0) {
@@ -334,37 +431,24 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
     for (; k + (U - 1) * T < row.nvec; k += U * T) {
       u32x4 raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = row.load(k + u * T);
+      for (int u = 0; u < U; ++u) raw[u] = row.template load<false>(k + u * T);
 #pragma unroll
       for (int u = 0; u < U; ++u) piece(k + u * T, raw[u]);
     }
-    for (; k < row.nvec; k += T) piece(k, row.load(k));
+    for (; k < row.nvec; k += T) piece(k, row.template load<false>(k));
   }
   __syncthreads();
-  // the named places again, by the first of the pairs with an id; the label's by thread 0 unless a pair has it
-  if (SOFT) {
-    for (int k = t; k < a.K; k += T) {
-      const int32_t id = tid_l[k];
+  // the named places again
+  if (has_soft(MODE)) {
+    for (int k = t; k <= a.K; k += T) {
+      const int32_t id = place[k];
       if (id < 0) continue;
-      float p = 0.f;
-      bool first = true;
-      for (int i = 0; i < a.K; ++i) {
-        if (tid_l[i] == id) {
-          first = first && i >= k;
-          p += tp_l[i];
-        }
-      }
-      if (!first) continue;
-      float g = dense(elem<DT>(z, id)) - c * a.sw * a.T * p;
-      if (HARD && id == y) g -= c * a.hw;
+      float g = dense(elem<DT>(z, id)) - c * a.sw * a.T * prob[k];
+      if (has_hard(MODE) && id == y) g -= c * a.hw;
       put<DT>(dz, id, g);
     }
-  }
-  if (HARD && t == 0 && !bad) {
-    bool named = false;
-    if (SOFT)
-      for (int i = 0; i < a.K; ++i) named |= tid_l[i] == y;
-    if (!named) put<DT>(dz, y, dense(elem<DT>(z, y)) - c * a.hw);
+  } else if (t == 0 && !bad) {
+    put<DT>(dz, y, dense(elem<DT>(z, y)) - c * a.hw);
   }
 }
 
@@ -376,10 +460,31 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* lo
   const int t = threadIdx.x;
   double s = 0.;
   int32_t n = 0;
-  for (int64_t r = t; r < a.rows; r += 1024) {
-    int64_t y;
-    if (SUM) s += a.row_loss[r];
-    n += row_label(a, r, y) ? 1 : 0;
+  // without a branch between the loads: U rows' in flight
+  const uint32_t rows = (uint32_t)a.rows, w = (uint32_t)a.label_bytes / 4, shift = (uint32_t)a.shift;
+  const int32_t* lab = (const int32_t*)a.labels;
+  constexpr int U = 8;
+  for (uint32_t r0 = t; r0 < rows; r0 += U * 1024) {
+    float x[U];
+    int32_t lo[U], hi[U];
+    bool last[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t r = min(r0 + u * 1024, rows - 1);
+      x[u] = SUM ? a.row_loss[r] : 0.f;
+      last[u] = shift && (r + 1) % shift == 0;
+      const uint64_t i = (uint64_t)(shift && !last[u] ? r + 1 : r) * w;
+      lo[u] = lab ? lab[i] : 0;
+      hi[u] = lab ? lab[i + w - 1] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t y = w == 2 ? (int64_t)((uint64_t)(uint32_t)hi[u] << 32 | (uint32_t)lo[u]) : (int64_t)lo[u];
+      if (r0 + u * 1024 < rows) {
+        s += x[u];
+        n += !lab || (!last[u] && y != a.ignore) ? 1 : 0;
+      }
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -400,40 +505,46 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* lo
   if (inv_count) *inv_count = 1.f / (float)n;
 }
 
-template <int DT, int PHASE, int T, int NC> static int run_loss(const LossArgs& a, hipStream_t s) {
+template <int DT, int PHASE, int T, int NC, int U> static int run_loss(const LossArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)a.rows), block(T);
-  if (a.sw == 0.f) hipLaunchKernelGGL((loss_row_kernel<DT, PHASE, true, false, T, NC>), grid, block, 0, s, a);
-  else if (a.hw == 0.f) hipLaunchKernelGGL((loss_row_kernel<DT, PHASE, false, true, T, NC>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((loss_row_kernel<DT, PHASE, true, true, T, NC>), grid, block, 0, s, a);
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, s, a); };
+  if (a.sw == 0.f) go(loss_row_kernel<DT, PHASE, HARD, T, NC, U>);
+  else if (a.hw == 0.f) go(loss_row_kernel<DT, PHASE, SOFT, T, NC, U>);
+  else if (a.T == 1.f) go(loss_row_kernel<DT, PHASE, BOTH_T1, T, NC, U>);
+  else if (a.T == 2.f) go(loss_row_kernel<DT, PHASE, BOTH_T2, T, NC, U>);
+  else go(loss_row_kernel<DT, PHASE, BOTH, T, NC, U>);
   return hipGetLastError() == hipSuccess ? 0 : -7;
 }
 
-// Threads a row by its pieces: a wave for short rows, four for longer ones; the step the fewest registers that hold the
+// Threads a row by its pieces: a wave for short rows, more for longer ones; the step the fewest registers that hold the
 // row in a workgroup.
 template <int DT, int PHASE> static int run_loss(const LossArgs& a, hipStream_t s) {
   const int pieces = a.V / Vec<DT>::N;
   if constexpr (PHASE == LOSS_STEP) {
-    if (pieces <= 64 * 4) return run_loss<DT, PHASE, 64, 4>(a, s);
-    if (pieces <= 256 * 4) return run_loss<DT, PHASE, 256, 4>(a, s);
-    if (pieces <= 512 * 4) return run_loss<DT, PHASE, 512, 4>(a, s);
-    if (pieces <= 512 * 8) return run_loss<DT, PHASE, 512, 8>(a, s);
-    if (pieces <= 1024 * 8) return run_loss<DT, PHASE, 1024, 8>(a, s);
-    if (pieces <= 1024 * 16) return run_loss<DT, PHASE, 1024, 16>(a, s);
-    return run_loss<DT, PHASE, 1024, 0>(a, s);
+    if (pieces <= 64 * 4) return run_loss<DT, PHASE, 64, 4, 1>(a, s);
+    if (pieces <= 256 * 4) return run_loss<DT, PHASE, 256, 4, 1>(a, s);
+    if (pieces <= 512 * 4) return run_loss<DT, PHASE, 512, 4, 1>(a, s);
+    if (pieces <= 512 * 8) return run_loss<DT, PHASE, 512, 8, 1>(a, s);
+    if (pieces <= 1024 * 8) return run_loss<DT, PHASE, 1024, 8, 1>(a, s);
+    if (pieces <= 1024 * 16) return run_loss<DT, PHASE, 1024, 16, 1>(a, s);
+    return run_loss<DT, PHASE, 1024, 0, 4>(a, s);
   } else {
-    if (pieces <= 64 * 4) return run_loss<DT, PHASE, 64, 0>(a, s);
-    return run_loss<DT, PHASE, 256, 0>(a, s);
+    if (pieces <= 64 * 4) return run_loss<DT, PHASE, 64, 0, 4>(a, s);
+    if (pieces <= 256 * 8) return run_loss<DT, PHASE, 256, 0, 4>(a, s);
+    if constexpr (PHASE == LOSS_BWD) return run_loss<DT, PHASE, 1024, 0, 3>(a, s);
+    else return run_loss<DT, PHASE, 512, 0, 4>(a, s);
   }
 }
 
 template <int DT> static int loss_phase(int phase, const LossArgs& a, hipStream_t s) {
-  if (phase == LOSS_FWD) return run_loss<DT, LOSS_FWD>(a, s);
   if (phase == LOSS_BWD) return run_loss<DT, LOSS_BWD>(a, s);
-  return run_loss<DT, LOSS_STEP>(a, s);
+  if (phase == LOSS_STEP) return run_loss<DT, LOSS_STEP>(a, s);
+  return a.stats ? run_loss<DT, LOSS_FWD>(a, s) : run_loss<DT, LOSS_ALONE>(a, s);
 }
 
-int launch_loss(int dtype, int phase, const LossArgs& a, hipStream_t s) {
+int launch_loss(int dtype, int phase, LossArgs a, hipStream_t s) {
   if (a.rows == 0) return 0;
+  a.stream = a.rows * a.V * (dtype == 1 ? 4 : 2) > STREAM_BYTES;
   if (dtype == 0) return loss_phase<0>(phase, a, s);
   if (dtype == 1) return loss_phase<1>(phase, a, s);
   return loss_phase<2>(phase, a, s);
