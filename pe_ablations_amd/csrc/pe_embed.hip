@@ -112,9 +112,26 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_fwd_kerne
 
 // ------------------------------------------------------------------ sorting the tokens
 // The key of a token: its id, or V (behind every row of the vocabulary) when its gradient goes nowhere.
-__device__ __forceinline__ int32_t token_key(const EmbedArgs& a, int64_t t) {
-  const int64_t id = load_id(a.ids, a.id_bytes, t);
+__device__ __forceinline__ int32_t id_key(const EmbedArgs& a, int64_t id) {
   return id < 0 || id >= a.V || id == a.pad ? (int32_t)a.V : (int32_t)id;
+}
+__device__ __forceinline__ int32_t token_key(const EmbedArgs& a, int64_t t) { return id_key(a, load_id(a.ids, a.id_bytes, t)); }
+// Keys of tokens t0, t0 + step, ... , -1 from a.n (> 0) on; both halves of every id are loaded ahead of any use.
+template <int M> __device__ __forceinline__ void token_keys(const EmbedArgs& a, int t0, int step, int32_t (&key)[M]) {
+  const int32_t* ids = (const int32_t*)a.ids;
+  const int w = a.id_bytes / 4, n = (int)a.n;
+  int32_t lo[M], hi[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    const int64_t at = (int64_t)min(t0 + i * step, n - 1) * w;
+    lo[i] = ids[at];
+    hi[i] = ids[at + w - 1];
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    const int64_t id = w == 2 ? (int64_t)((uint64_t)(uint32_t)hi[i] << 32 | (uint32_t)lo[i]) : (int64_t)lo[i];
+    key[i] = t0 + i * step < n ? id_key(a, id) : -1;
+  }
 }
 
 // no token of any id yet: thread i of `n`
@@ -122,68 +139,15 @@ __device__ __forceinline__ void clear_runs(const EmbedArgs& a, int64_t i, int64_
   for (; i < a.V; i += n) a.run[i] = int2{0, 0};
 }
 
-__global__ __launch_bounds__(256) void embed_clear_kernel(EmbedArgs a) {
-  clear_runs(a, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
-}
-
-// Up to RANK_MAX tokens, in one launch: a token's place is the number of tokens with a smaller key, or the same key and
-// an earlier position.  A wave holds RANK_KEYS keys, 64 a register, and compares a register with one token's key at a
-// time: one vector comparison and two scalar instructions for 64 pairs.  Tokens of earlier registers come first at
-// equal keys, which is a comparison with key + 1; the token's own register takes its equal lanes below it as well.
-constexpr int RANK_MAX = 16384, RANK_KEYS = 4096, RANK_WAVES = 8;
-
-__global__ __launch_bounds__(RANK_WAVES * 64) void embed_rank_kernel(EmbedArgs a, int per_wave) {
-  __shared__ int32_t keys[RANK_KEYS];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = (int)a.n;
-  const int t0 = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * RANK_WAVES + w) * per_wave);
-  clear_runs(a, (int64_t)blockIdx.x * (RANK_WAVES * 64) + threadIdx.x, (int64_t)gridDim.x * (RANK_WAVES * 64));
-  int32_t mine = 0x7fffffff;  // lane i: the key and the place of token t0 + i
-  if (lane < per_wave && t0 + lane < n) mine = token_key(a, t0 + lane);
-  int32_t place = 0;
-  for (int u0 = 0; u0 < n; u0 += RANK_KEYS) {
-    __syncthreads();
-    int32_t x[RANK_KEYS / (RANK_WAVES * 64)];  // every load ahead of the first store
-#pragma unroll
-    for (int i = 0; i < RANK_KEYS / (RANK_WAVES * 64); ++i) {
-      const int u = u0 + i * (RANK_WAVES * 64) + threadIdx.x;
-      x[i] = token_key(a, min(u, n - 1));
-      x[i] = u < n ? x[i] : 0x7fffffff;
-    }
-#pragma unroll
-    for (int i = 0; i < RANK_KEYS / (RANK_WAVES * 64); ++i) keys[i * (RANK_WAVES * 64) + threadIdx.x] = x[i];
-    __syncthreads();
-    int32_t k[RANK_KEYS / 64];
-#pragma unroll
-    for (int j = 0; j < RANK_KEYS / 64; ++j) k[j] = keys[j * 64 + lane];
-    const int regs = min(RANK_KEYS, n - u0 + 63) / 64;
-    for (int i = 0; i < per_wave && t0 + i < n; ++i) {
-      const int t = t0 + i, own = (t >> 6) - (u0 >> 6);
-      const int32_t key = __builtin_amdgcn_readlane(mine, i);
-      int cnt = 0;
-#pragma unroll
-      for (int j = 0; j < RANK_KEYS / 64; ++j) {
-        if (j % 8 == 0 && j >= regs) break;
-        cnt += __popcll(__ballot(k[j] < key + (j < own ? 1 : 0)));
-      }
-      if (own >= 0 && own < RANK_KEYS / 64)
-        cnt += __popcll(__ballot(keys[own * 64 + lane] == key) & ((1ull << (t & 63)) - 1));
-      place += lane == i ? cnt : 0;
-    }
-  }
-  if (lane < per_wave && t0 + lane < n) {
-    a.key[place] = mine;
-    a.order[place] = t0 + lane;
-  }
-}
-
-// More tokens: least significant digits first, `bits` of them a pass, tiles of 1024 tokens.  A pass counts each
-// tile's digits, turns the counts into each tile's place within its digit, and moves the tokens.
-constexpr int TILE = 1024, MAXBITS = 10;
+// Least significant digits first, `bits` of them a pass, tiles of 1024 tokens.  A pass counts each tile's digits, turns
+// the counts into each tile's place within its digit, and moves the tokens.  Up to FEW_TILES tiles add up the counts
+// of those before them where they move the tokens; a launch of its own does so for more.
+constexpr int TILE = 1024, MAXBITS = 10, FEW_TILES = 64;
 
 struct SortArgs {
   const int32_t *key_in, *order_in;  // NULL in the first pass, which takes the tokens themselves
   int32_t *key_out, *order_out;
-  int32_t *hist;                     // [tiles][bins], then each tile's offset within the bin
+  int32_t *hist;                     // [tiles][bins], past FEW_TILES tiles then each one's offset within the bin
   int32_t *total;                    // [bins]
   int tiles, shift, bits;
 };
@@ -233,7 +197,20 @@ __global__ __launch_bounds__(TILE) void embed_scatter_kernel(EmbedArgs a, SortAr
   const int bins = 1 << s.bits, t = threadIdx.x, lane = t & 63, w = t >> 6;
   const int64_t i = (int64_t)blockIdx.x * TILE + t;
   // where each digit begins: an exclusive sum of the totals over the bins, one bin a thread
-  const int32_t tot = t < bins ? s.total[t] : 0;
+  int32_t tot = 0, ahead = 0;
+  if (t < bins) {
+    if (s.tiles <= FEW_TILES) {
+#pragma unroll 16
+      for (int k = 0; k < s.tiles; ++k) {
+        const int32_t x = s.hist[k * bins + t];
+        tot += x;
+        ahead += k < (int)blockIdx.x ? x : 0;
+      }
+    } else {
+      tot = s.total[t];
+      ahead = s.hist[(int64_t)blockIdx.x * bins + t];
+    }
+  }
   int32_t inc = tot;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -245,7 +222,7 @@ __global__ __launch_bounds__(TILE) void embed_scatter_kernel(EmbedArgs a, SortAr
   __syncthreads();
   int32_t before = 0;
   for (int k = 0; k < w; ++k) before += wsum[k];
-  if (t < bins) base[t] = before + inc - tot + s.hist[(int64_t)blockIdx.x * bins + t];
+  if (t < bins) base[t] = before + inc - tot + ahead;
   const bool live = i < a.n;
   const int32_t key = live ? sort_key(a, s, i) : 0;
   const int d = (key >> s.shift) & (bins - 1);
@@ -339,26 +316,21 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_chunk_ker
 constexpr int SHORT_RUN = 32;  // tokens that one group of lanes adds up alone
 constexpr int MAX_ROWS = 64;   // rows of the vocabulary a workgroup takes
 
-// Rows v = bx + j (int)(gridDim.x / a.slices): frequent ids are neighbours, and so are shared out.  Each group of lanes takes the
-// workgroup's rows with short runs in turn; then the workgroup adds up each long run together, as the tokens ahead of
-// its first whole chunk, the chunks' sums, and the tokens behind the last, cut into as many equal parts as there
-// are groups, whose sums are added in order.
-template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedArgs a) {
+// The gradient's rows v = bx + j G, j < nr, of one workgroup from their runs of tokens: frequent ids are neighbours, and
+// so are shared out.  Each group of lanes takes the rows with short runs in turn; then the workgroup adds up each long
+// run together, as the tokens ahead of its first whole chunk, the chunks' sums (CHUNKS), and the tokens behind the
+// last, cut into as many equal parts as there are groups, whose sums are added in order.
+template <int DT, int VB, bool CHUNKS, class O>
+__device__ __forceinline__ void grad_rows(const EmbedArgs& a, int slice, int bx, int64_t G, int nr, const int2* run, float* red, O order) {
   using P = Piece<DT, VB>;
-  const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;
-  __shared__ int2 run[MAX_ROWS];
-  __shared__ float red[256 * P::N];
-  const int G = (int)(gridDim.x / a.slices), nr = (int)((a.V - bx + G - 1) / G);
-  if (threadIdx.x < nr) run[threadIdx.x] = a.run[bx + threadIdx.x * (int64_t)G];
-  __syncthreads();
   const int sub = threadIdx.x & (a.lpr - 1), grp = threadIdx.x / a.lpr, ng = 256 / a.lpr;
   const int c = slice * a.lpr + sub;
   const int64_t col = (int64_t)c * VB;
-  auto token = [&](int64_t i) { return (int64_t)a.order[i] * a.x_rs * P::ES; };
+  auto token = [&](int64_t i) { return (int64_t)order(i) * a.x_rs * P::ES; };
   auto put = [&](int j, float (&s)[P::N]) {
 #pragma unroll
     for (int e = 0; e < P::N; ++e) s[e] = product(s[e], a.scale);
-    P::store(a.y, (bx + j * (int64_t)G) * a.y_rs * P::ES + col, s);
+    P::store(a.y, (bx + j * G) * a.y_rs * P::ES + col, s);
   };
   if (c < a.pieces) {
     for (int j = grp; j < nr; j += ng) {
@@ -373,7 +345,7 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_kerne
     const int32_t i0 = run[j].x, i1 = run[j].y;
     if (i1 - i0 <= SHORT_RUN) continue;
     // items: [0, h) tokens i0.., [h, h + m) chunks k0.., [h + m, total) tokens behind the last chunk
-    const int32_t k0 = (i0 + a.chunk - 1) / a.chunk, k1 = i1 / a.chunk;
+    const int32_t k0 = CHUNKS ? (i0 + a.chunk - 1) / a.chunk : 0, k1 = CHUNKS ? i1 / a.chunk : 0;
     const bool chunks = k1 > k0;
     const int32_t h = chunks ? k0 * a.chunk - i0 : i1 - i0, m = chunks ? k1 - k0 : 0;
     const int32_t total = chunks ? h + m + (i1 - k1 * a.chunk) : h;
@@ -381,11 +353,13 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_kerne
     float s[P::N] = {};
     if (c < a.pieces) {
       add_rows<DT, VB>(a.x, col, i0 + min(b0, h), i0 + min(b1, h), token, s);
-      for (int32_t k = k0 + min(max(b0 - h, 0), m); k < k0 + min(max(b1 - h, 0), m); ++k)
+      if (chunks) {
+        for (int32_t k = k0 + min(max(b0 - h, 0), m); k < k0 + min(max(b1 - h, 0), m); ++k)
 #pragma unroll
-        for (int e = 0; e < P::N; ++e) s[e] += a.part[(int64_t)k * a.H + (int64_t)c * P::N + e];
-      const int64_t q = (int64_t)k1 * a.chunk - h - m;  // item b behind the chunks is token q + b
-      if (chunks) add_rows<DT, VB>(a.x, col, q + max(b0, h + m), q + max(b1, h + m), token, s);
+          for (int e = 0; e < P::N; ++e) s[e] += a.part[(int64_t)k * a.H + (int64_t)c * P::N + e];
+        const int64_t q = (int64_t)k1 * a.chunk - h - m;  // item b behind the chunks is token q + b
+        add_rows<DT, VB>(a.x, col, q + max(b0, h + m), q + max(b1, h + m), token, s);
+      }
     }
     __syncthreads();
 #pragma unroll
@@ -398,6 +372,84 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_kerne
       put(j, s);
     }
   }
+}
+
+template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedArgs a) {
+  const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;
+  __shared__ int2 run[MAX_ROWS];
+  __shared__ float red[256 * Piece<DT, VB>::N];
+  const int64_t G = gridDim.x / a.slices;
+  const int nr = (int)((a.V - bx + G - 1) / G);
+  if (threadIdx.x < nr) run[threadIdx.x] = a.run[bx + threadIdx.x * G];
+  __syncthreads();
+  grad_rows<DT, VB, true>(a, slice, bx, G, nr, run, red, [&](int64_t i) { return a.order[i]; });
+}
+
+// Up to FEW tokens, in one launch without a workspace: every workgroup picks the tokens of its own rows from all of them
+// (G a power of two: row j of token id has id = bx + j G), in order, by a ballot for 64 tokens, and then lists each
+// row's in turn.
+constexpr int FEW = 4096;
+
+template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_few_kernel(EmbedArgs a, int log_g) {
+  constexpr int N = Piece<DT, VB>::N;
+  const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;
+  __shared__ int2 run[MAX_ROWS];
+  __shared__ uint16_t order[FEW];
+  __shared__ union { uint32_t list[FEW]; float red[256 * N]; } u;  // j << 16 | token; the sums come after its last use
+  __shared__ int32_t count[4];
+  const int64_t G = (int64_t)1 << log_g;
+  const int nr = (int)((a.V - bx + G - 1) / G), n = (int)a.n;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint64_t below = (1ull << lane) - 1;
+  // wave w takes a quarter of the tokens, in whole steps of 64
+  constexpr int STEPS = FEW / 256;
+  const int steps = (n + 255) / 256, s0 = w * steps * 64;
+  int32_t key[STEPS];
+  if (n > 0) {
+    token_keys(a, s0 + lane, 64, key);
+  } else {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) key[i] = -1;
+  }
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    if (i >= steps || key[i] >= (int32_t)a.V || (key[i] & (int32_t)(G - 1)) != bx) key[i] = -1;
+    mine += __popcll(__ballot(key[i] >= 0));
+  }
+  if (lane == 0) count[w] = mine;
+  __syncthreads();
+  int at = 0;
+  for (int i = 0; i < w; ++i) at += count[i];
+  const int total = count[0] + count[1] + count[2] + count[3];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const uint64_t m = __ballot(key[i] >= 0);
+    if (key[i] >= 0) u.list[at + __popcll(m & below)] = (uint32_t)(key[i] >> log_g) << 16 | (uint32_t)(s0 + i * 64 + lane);
+    at += __popcll(m);
+  }
+  __syncthreads();
+  // the tokens of each row: wave w lists rows w, w + 4, ...; the rows before it say where it begins
+  for (int j = w; j < nr; j += 4) {
+    int before = 0, len = 0;
+    for (int i = lane; i < (total + 63) / 64 * 64; i += 64) {
+      const uint32_t x = i < total ? u.list[i] : 0xffffffffu;
+      before += __popcll(__ballot((int)(x >> 16) < j));
+      len += __popcll(__ballot((int)(x >> 16) == j));
+    }
+    if (len) {
+      int pos = before;
+      for (int i = lane; i < (total + 63) / 64 * 64; i += 64) {
+        const uint32_t x = i < total ? u.list[i] : 0xffffffffu;
+        const uint64_t m = __ballot((int)(x >> 16) == j);
+        if ((int)(x >> 16) == j) order[pos + __popcll(m & below)] = (uint16_t)x;
+        pos += __popcll(m);
+      }
+    }
+    if (lane == 0) run[j] = int2{before, before + len};
+  }
+  __syncthreads();
+  grad_rows<DT, VB, false>(a, slice, bx, G, nr, run, u.red, [&](int64_t i) { return (int32_t)order[i]; });
 }
 
 namespace {
@@ -445,6 +497,9 @@ int key_bits(int64_t V) {  // of keys 0 .. V
   return b;
 }
 
+// a grid's threads are counted in 32 bits
+bool grid_fits(int64_t blocks, int threads) { return blocks * threads <= 0xffffffffll; }
+
 int done() { return hipGetLastError() == hipSuccess ? 0 : -7; }
 
 }  // namespace
@@ -455,66 +510,72 @@ int launch_embed_fwd(int dtype, EmbedArgs a, hipStream_t s) {
   a.lpr = lanes_per_row(a.pieces, 256);
   const int64_t rows = (int64_t)(256 / a.lpr) * LOOKUP_ROWS;
   const dim3 grid((unsigned)((a.n + rows - 1) / rows)), block(256);
+  if (!grid_fits((a.n + rows - 1) / rows, 256)) return -2;
   return with_piece(dtype, vb, [&](auto dt, auto v) {
     hipLaunchKernelGGL((embed_fwd_kernel<decltype(dt)::value, decltype(v)::value>), grid, block, 0, s, a);
     return done();
   });
 }
 
-// each id's run; [key][order] of the sorted tokens; past RANK_MAX tokens a second pair and the counts; the chunks' sums
+// past FEW tokens: each id's run; [key][order] of the sorted tokens, twice; the digits' counts; the chunks' sums
 int64_t embed_bwd_workspace(int64_t n, int64_t V, int H) {
-  int64_t w = up4(2 * V) + 2 * up4(n);
-  if (n > RANK_MAX) w += 2 * up4(n) + ((n + TILE - 1) / TILE + 1) * (1 << MAXBITS);
-  return 4 * (w + n / chunk_tokens(n) * (int64_t)H) + 16;
+  if (n <= FEW) return 16;
+  return 4 * (up4(2 * V) + 4 * up4(n) + (((n + TILE - 1) / TILE + 1) << MAXBITS) + n / chunk_tokens(n) * (int64_t)H) + 16;
 }
 
 int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s) {
   const int es = dtype == 1 ? 4 : 2, vb = piece_bytes(es, a);
+  a.pieces = (int)((int64_t)a.H * es / vb);
+  // Lanes on a row: a whole workgroup where most rows of the gradient are zeros, so that the tokens are picked for
+  // all of its columns at once; else a wave, whose slices and groups share the long runs (fp32 50257 x 512, 4096
+  // tokens: 29 against 37 us; bf16 2000 x 1024, 4096 tokens: 24 against 18 us)
+  a.lpr = lanes_per_row(a.pieces, a.n <= FEW && a.V >= 4 * a.n ? 256 : 64);
+  a.slices = (a.pieces + a.lpr - 1) / a.lpr;
+  if (a.n <= FEW) {
+    // 15 to 30 rows a workgroup, fewer where that leaves compute units idle
+    int log_g = 0;
+    while (((int64_t)15 << (log_g + 1)) <= a.V || (log_g < 9 && ((int64_t)2 << log_g) <= a.V)) ++log_g;
+    if (!grid_fits((int64_t)a.slices << log_g, 256)) return -2;
+    return with_piece(dtype, vb, [&](auto dt, auto v) {
+      hipLaunchKernelGGL((embed_bwd_few_kernel<decltype(dt)::value, decltype(v)::value>), dim3((unsigned)a.slices << log_g),
+                         dim3(256), 0, s, a, log_g);
+      return done();
+    });
+  }
   int32_t* p = (int32_t*)ws;
   auto take = [&](int64_t n) { int32_t* q = p; p += n; return q; };
   a.run = (int2*)take(up4(2 * a.V));
   a.key = take(up4(a.n));
   a.order = take(up4(a.n));
-  if (a.n > RANK_MAX) {
-    int32_t *key2 = take(up4(a.n)), *order2 = take(up4(a.n));
-    SortArgs o;
-    o.tiles = (int)((a.n + TILE - 1) / TILE);
-    o.hist = take((int64_t)o.tiles << MAXBITS);
-    o.total = take(1 << MAXBITS);
-    const int bits = key_bits(a.V), passes = (bits + MAXBITS - 1) / MAXBITS;
-    o.bits = (bits + passes - 1) / passes;
-    for (int i = 0; i < passes; ++i) {
-      const bool last_in_first = (passes - 1 - i) % 2 == 0;  // the last pass writes a.key / a.order
-      o.key_in = i == 0 ? nullptr : (last_in_first ? key2 : a.key);
-      o.order_in = i == 0 ? nullptr : (last_in_first ? order2 : a.order);
-      o.key_out = last_in_first ? a.key : key2;
-      o.order_out = last_in_first ? a.order : order2;
-      o.shift = i * o.bits;
-      hipLaunchKernelGGL(embed_hist_kernel, dim3(o.tiles), dim3(TILE), 0, s, a, o);
+  int32_t *key2 = take(up4(a.n)), *order2 = take(up4(a.n));
+  SortArgs o;
+  o.tiles = (int)((a.n + TILE - 1) / TILE);
+  o.hist = take((int64_t)o.tiles << MAXBITS);
+  o.total = take(1 << MAXBITS);
+  const int bits = key_bits(a.V), passes = (bits + MAXBITS - 1) / MAXBITS;
+  o.bits = (bits + passes - 1) / passes;
+  for (int i = 0; i < passes; ++i) {
+    const bool last_in_first = (passes - 1 - i) % 2 == 0;  // the last pass writes a.key / a.order
+    o.key_in = i == 0 ? nullptr : (last_in_first ? key2 : a.key);
+    o.order_in = i == 0 ? nullptr : (last_in_first ? order2 : a.order);
+    o.key_out = last_in_first ? a.key : key2;
+    o.order_out = last_in_first ? a.order : order2;
+    o.shift = i * o.bits;
+    hipLaunchKernelGGL(embed_hist_kernel, dim3(o.tiles), dim3(TILE), 0, s, a, o);
+    if (o.tiles > FEW_TILES)
       hipLaunchKernelGGL(embed_scan_kernel, dim3(((1 << o.bits) + 31) / 32), dim3(1024), 0, s, o);
-      hipLaunchKernelGGL(embed_scatter_kernel, dim3(o.tiles), dim3(TILE), 0, s, a, o);
-    }
-  } else if (a.n) {
-    // about one workgroup per compute unit
-    const int per_wave = std::max(1, (int)((a.n + 256 * RANK_WAVES - 1) / (256 * RANK_WAVES)));
-    const int64_t per = (int64_t)per_wave * RANK_WAVES;
-    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((a.n + per - 1) / per)), dim3(RANK_WAVES * 64), 0, s, a, per_wave);
-  } else {
-    hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)((a.V + 255) / 256)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(embed_scatter_kernel, dim3(o.tiles), dim3(TILE), 0, s, a, o);
   }
   if (hipGetLastError() != hipSuccess) return -7;
   a.part = (float*)p;
   a.chunk = chunk_tokens(a.n);
-  a.pieces = (int)((int64_t)a.H * es / vb);
-  a.lpr = lanes_per_row(a.pieces, 64);
-  a.slices = (a.pieces + a.lpr - 1) / a.lpr;
   const unsigned chunks = (unsigned)((a.n + a.chunk - 1) / a.chunk);
   const unsigned rows = (unsigned)((a.V + MAX_ROWS - 1) / MAX_ROWS);
   const unsigned grid = (unsigned)std::min<int64_t>(a.V, std::max<int64_t>(rows, 1024));
-  if ((int64_t)std::max(grid, chunks) * a.slices > 0x7fffffff) return -2;
+  if (!grid_fits((int64_t)std::max(grid, chunks) * a.slices, 256)) return -2;
   return with_piece(dtype, vb, [&](auto dt, auto v) {
     constexpr int D = decltype(dt)::value, B = decltype(v)::value;
-    if (chunks) hipLaunchKernelGGL((embed_chunk_kernel<D, B>), dim3(chunks * a.slices), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((embed_chunk_kernel<D, B>), dim3(chunks * a.slices), dim3(256), 0, s, a);
     hipLaunchKernelGGL((embed_bwd_kernel<D, B>), dim3(grid * a.slices), dim3(256), 0, s, a);
     return done();
   });

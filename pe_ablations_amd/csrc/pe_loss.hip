@@ -507,6 +507,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* lo
 
 template <int DT, int PHASE, int T, int NC, int U> static int run_loss(const LossArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)a.rows), block(T);
+  if (a.rows * T > 0xffffffffll) return -2;  // a grid's threads are counted in 32 bits
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, s, a); };
   if (a.sw == 0.f) go(loss_row_kernel<DT, PHASE, HARD, T, NC, U>);
   else if (a.hw == 0.f) go(loss_row_kernel<DT, PHASE, SOFT, T, NC, U>);
