@@ -29,7 +29,8 @@ int pe_embed_fwd(const void* ids, int32_t id_bytes, int64_t n, const void* weigh
 
 /* Its weight gradient: dweight[v] = scale * sum of dy[t] over the t with ids[t] == v, in increasing t, for every v
  * of the vocabulary (0 where no token has it, and for v == padding_idx; pass -1 for none).  ids outside
- * [0, vocab) add nothing.  The workspace holds the tokens sorted by id.  n <= 2^24. */
+ * [0, vocab) add nothing.  The workspace holds the tokens sorted by id; up to 4096 tokens need none (0 bytes, NULL).
+ * n <= 2^24. */
 size_t pe_embed_bwd_workspace_bytes(int64_t n, int64_t vocab, int32_t dim);
 int pe_embed_bwd(const void* ids, int32_t id_bytes, int64_t n, const void* dy, int32_t dtype, int64_t dy_row_stride,
                  int64_t vocab, int32_t dim, float scale, int64_t padding_idx, void* dweight,

@@ -519,7 +519,7 @@ int launch_embed_fwd(int dtype, EmbedArgs a, hipStream_t s) {
 
 // past FEW tokens: each id's run; [key][order] of the sorted tokens, twice; the digits' counts; the chunks' sums
 int64_t embed_bwd_workspace(int64_t n, int64_t V, int H) {
-  if (n <= FEW) return 16;
+  if (n <= FEW) return 0;
   return 4 * (up4(2 * V) + 4 * up4(n) + (((n + TILE - 1) / TILE + 1) << MAXBITS) + n / chunk_tokens(n) * (int64_t)H) + 16;
 }
 

@@ -80,7 +80,8 @@ int pe_embed_bwd(const void* ids, int32_t id_bytes, int64_t n, const void* dy, i
   if (rc) return rc;
   if (n > (1 << 24) || padding_idx < -1 || padding_idx >= vocab) return PE_ERR_SHAPE;
   if (!dweight || (n && (!ids || !dy))) return PE_ERR_NULL;
-  if (!workspace || !aligned(workspace, 16) || ws_bytes < pe_embed_bwd_workspace_bytes(n, vocab, dim)) return PE_ERR_WORKSPACE;
+  const size_t need = pe_embed_bwd_workspace_bytes(n, vocab, dim);
+  if (need && (!workspace || !aligned(workspace, 16) || ws_bytes < need)) return PE_ERR_WORKSPACE;
   if ((rc = pe::device_ready())) return rc;
   pe::EmbedArgs a;
   memset(&a, 0, sizeof(a));

@@ -11,9 +11,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .functional import _dtype_code, _expression_grads, _on, _stream, plain_autograd
+from .functional import _dtype_code, _expression_grads, _on, _ptr, _stream, plain_autograd
 
 _FLOATS = (torch.bfloat16, torch.float32, torch.float16)
+_INTS = (torch.int64, torch.int32)
 _MAX_TOKENS = 1 << 24
 
 
@@ -21,37 +22,60 @@ def _check(ids: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[int]) 
     """The checks of an embedding call; padding_idx as the C ABI takes it (-1 for none)."""
     if not weight.is_cuda:
         raise RuntimeError("embedding runs on the GPU only (got a CPU weight)")
-    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+    if weight.dim() != 2:
         raise ValueError(f"embedding: weight must be (vocab, dim), got shape {tuple(weight.shape)}")
-    if weight.dtype not in _FLOATS:
-        raise TypeError(f"embedding supports bf16 / fp16 / fp32 weights, got {weight.dtype}")
-    if ids.dtype not in (torch.int64, torch.int32):
+    return _check_parts(ids, weight.shape[0], weight.shape[1], weight.dtype, weight.device, padding_idx)
+
+
+def _check_parts(ids, V: int, H: int, dtype: torch.dtype, dev: torch.device, padding_idx: Optional[int]) -> int:
+    if V <= 0 or H <= 0:
+        raise ValueError(f"embedding: the weight must have rows and columns, got ({V}, {H})")
+    if dtype not in _FLOATS:
+        raise TypeError(f"embedding supports bf16 / fp16 / fp32 weights, got {dtype}")
+    if ids.dtype not in _INTS:
         raise TypeError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
-    if ids.device != weight.device:
-        raise ValueError(f"embedding: ids are on {ids.device}, the weight on {weight.device}")
+    if ids.device != dev:
+        raise ValueError(f"embedding: ids are on {ids.device}, the weight on {dev}")
     if padding_idx is None:
         return -1
-    V = weight.shape[0]
     if not -V <= padding_idx < V:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside a vocabulary of {V}")
     return padding_idx % V
 
 
+def _rows(t: torch.Tensor, H: int) -> torch.Tensor:
+    """A (rows, H) tensor that the library can read: unit stride, rows not overlapping (one row may have any)."""
+    return t if t.stride(1) == 1 and t.stride(0) >= H else t.contiguous()
+
+
 def _lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
     V, H = weight.shape
-    if weight.stride(1) != 1 or weight.stride(0) < H:
-        weight = weight.contiguous()
-    ids = ids.contiguous()
-    out = torch.empty(ids.shape + (H,), dtype=weight.dtype, device=weight.device)
+    weight, ids = _rows(weight, H), ids.contiguous()
+    dev = weight.device
+    out = torch.empty(ids.shape + (H,), dtype=weight.dtype, device=dev)
     n = ids.numel()
     if n:
-        dev = weight.device
         with _on(dev):
             rc = _lib.lib().pe_embed_fwd(ids.data_ptr(), ids.element_size(), n, weight.data_ptr(),
-                                         _dtype_code(weight.dtype), V, H, weight.stride(0), scale, out.data_ptr(), H,
+                                         _dtype_code(weight.dtype), V, H, max(weight.stride(0), H), scale, out.data_ptr(), H,
                                          _stream(dev))
         _lib.check(rc)
     return out
+
+
+def _gradient(ids: torch.Tensor, dy: torch.Tensor, V: int, scale: float, pad: int) -> torch.Tensor:
+    """embedding_backward on checked arguments (pad: -1 for none)."""
+    H, n, dev = dy.shape[-1], ids.numel(), dy.device
+    dy, ids = _rows(dy.reshape(-1, H), H), ids.contiguous()
+    dw = torch.empty((V, H), dtype=dy.dtype, device=dev)
+    L = _lib.lib()
+    nb = L.pe_embed_bwd_workspace_bytes(n, V, H)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None  # held until the launch is enqueued
+    with _on(dev):
+        rc = L.pe_embed_bwd(ids.data_ptr(), ids.element_size(), n, dy.data_ptr(), _dtype_code(dy.dtype),
+                            max(dy.stride(0), H), V, H, scale, pad, dw.data_ptr(), H, _ptr(ws), nb, _stream(dev))
+    _lib.check(rc)
+    return dw
 
 
 def embedding_backward(ids: torch.Tensor, dy: torch.Tensor, vocab_size: int, *, scale: float = 1.0,
@@ -61,28 +85,12 @@ def embedding_backward(ids: torch.Tensor, dy: torch.Tensor, vocab_size: int, *, 
     tokens, in fp32 (bitwise reproducible).  padding_idx's row is 0; ids outside the vocabulary add nothing."""
     if not dy.is_cuda:
         raise RuntimeError("embedding_backward runs on the GPU only (got a CPU tensor)")
-    if tuple(dy.shape[:-1]) != tuple(ids.shape) or dy.dim() != ids.dim() + 1:
+    if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape:
         raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} must be ids {tuple(ids.shape)} plus a last dim")
-    H = dy.shape[-1]
-    n = ids.numel()
-    if n > _MAX_TOKENS:
-        raise ValueError(f"embedding_backward: {n} tokens in one call, at most {_MAX_TOKENS} are supported")
-    dev = dy.device
-    dw = torch.empty((vocab_size, H), dtype=dy.dtype, device=dev)
-    pad = _check(ids, dw, padding_idx)
-    dy = dy.reshape(-1, H)
-    if dy.stride(1) != 1 or dy.stride(0) < H:
-        dy = dy.contiguous()
-    ids = ids.contiguous()
-    L = _lib.lib()
-    nb = L.pe_embed_bwd_workspace_bytes(n, vocab_size, H)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = L.pe_embed_bwd(ids.data_ptr(), ids.element_size(), n, dy.data_ptr(), _dtype_code(dy.dtype),
-                            max(dy.stride(0), H), vocab_size, H, scale, pad, dw.data_ptr(), H, ws.data_ptr(), nb,
-                            _stream(dev))
-    _lib.check(rc)
-    return dw
+    if ids.numel() > _MAX_TOKENS:
+        raise ValueError(f"embedding_backward: {ids.numel()} tokens in one call, at most {_MAX_TOKENS} are supported")
+    pad = _check_parts(ids, vocab_size, dy.shape[-1], dy.dtype, dy.device, padding_idx)
+    return _gradient(ids, dy, vocab_size, float(scale), pad)
 
 
 class EmbeddingFn(torch.autograd.Function):
@@ -90,18 +98,18 @@ class EmbeddingFn(torch.autograd.Function):
     backward differentiates F.embedding(ids, weight) * scale (as RMSNormFn)."""
 
     @staticmethod
-    def forward(ctx, weight, ids, scale, padding_idx):
+    def forward(ctx, weight, ids, scale, pad):
         ctx.save_for_backward(weight, ids)
-        ctx.scale, ctx.padding_idx = scale, padding_idx
+        ctx.scale, ctx.pad = scale, pad
         return _lookup(ids, weight, scale)
 
     @staticmethod
     def backward(ctx, dy):
         weight, ids = ctx.saved_tensors
         if torch.is_grad_enabled() or not plain_autograd(dy):
-            return _expression_grads(lambda: F.embedding(ids, weight, ctx.padding_idx) * ctx.scale, (weight,), ctx,
-                                     dy) + (None, None, None)
-        return embedding_backward(ids, dy, weight.shape[0], scale=ctx.scale, padding_idx=ctx.padding_idx), None, None, None
+            return _expression_grads(lambda: F.embedding(ids, weight, None if ctx.pad < 0 else ctx.pad) * ctx.scale,
+                                     (weight,), ctx, dy) + (None, None, None)
+        return _gradient(ids, dy, weight.shape[0], ctx.scale, ctx.pad), None, None, None
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
@@ -111,10 +119,10 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     the weight (embedding_backward); the rows of padding_idx get no gradient.  An id outside the vocabulary
     cannot be refused without waiting for the GPU: its row is NaN."""
     pad = _check(ids, weight, padding_idx)
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if weight.requires_grad and torch.is_grad_enabled():
         if ids.numel() > _MAX_TOKENS:
             raise ValueError(f"embedding: {ids.numel()} tokens in one call with gradients, at most {_MAX_TOKENS}")
-        return EmbeddingFn.apply(weight, ids, float(scale), None if pad < 0 else pad)
+        return EmbeddingFn.apply(weight, ids, float(scale), pad)
     return _lookup(ids, weight, float(scale))
 
 

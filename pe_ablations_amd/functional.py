@@ -177,10 +177,14 @@ def _stream(dev: torch.device):
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_NO_CONTEXT = contextlib.nullcontext()
+
+
 def _on(dev: torch.device):
-    """Make dev current for the library call (a no-op context when it already is)."""
-    if dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    """Make dev, a device of a CUDA tensor, current for the library call (a no-op context when it already is)."""
+    if dev.index == _current_device():
+        return _NO_CONTEXT
     return torch.cuda.device(dev)
 
 

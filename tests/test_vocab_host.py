@@ -108,10 +108,11 @@ def test_embed_entry_points_refuse(lib):
     assert fwd(ws=7) == fwd(os_=7) == fwd(ids=60) == fwd(w=129) == E["PE_ERR_STRIDE"]
     assert fwd(n=0) == E["PE_OK"]
 
-    nb = lib.pe_embed_bwd_workspace_bytes(5, 7, 8)
+    nb = lib.pe_embed_bwd_workspace_bytes(5000, 7, 8)
     assert nb > 0 and lib.pe_embed_bwd_workspace_bytes((1 << 24) + 1, 7, 8) == 0
+    assert lib.pe_embed_bwd_workspace_bytes(4096, 7, 8) == 0  # a few tokens need none
 
-    def bwd(ids=64, n=5, dy=128, V=7, pad=-1, dw=256, ws=512, wb=nb, stride=8):
+    def bwd(ids=64, n=5000, dy=128, V=7, pad=-1, dw=256, ws=512, wb=nb, stride=8):
         return lib.pe_embed_bwd(ids, 8, n, dy, 0, stride, V, 8, 1.0, pad, dw, 8, ws, wb, None)
     assert bwd(ids=None) == bwd(dy=None) == bwd(dw=None) == E["PE_ERR_NULL"]
     assert bwd(pad=7) == bwd(pad=-2) == bwd(n=(1 << 24) + 1) == E["PE_ERR_SHAPE"]
