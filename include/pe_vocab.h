@@ -59,7 +59,7 @@ typedef struct {
   int64_t ignore_index;
   int64_t teacher_id_stride; /* elements between rows of the teacher's ids / logits */
   int64_t teacher_row_stride;
-  int32_t vocab;
+  int32_t vocab;             /* at most 2^28 */
   int32_t dtype;             /* PE_DTYPE_* of logits and gradient */
   int32_t label_bytes;       /* 4 or 8 */
   int32_t reduction;         /* PE_LOSS_* */

@@ -82,29 +82,30 @@ template <int DT> struct Vec {
 };
 
 // A row of V elements at `p`: `head` single elements, `nvec` pieces of 16 bytes, and single elements to the end.
-// single(t) is the single element of thread t, or -1.
+// single(t) is the single element of thread t, or -1.  A piece's place is an unsigned 32-bit offset from a base that
+// is the same for every thread (rows below 4 GB), which takes one register where an address takes two.
 template <int DT> struct Row {
-  const char* p;
+  const char* body;
   int V, head, nvec;
-  __device__ __forceinline__ Row(const char* q, int v) : p(q), V(v) {
+  __device__ __forceinline__ Row(const char* p, int v) : V(v) {
     constexpr int ES = Vec<DT>::ES;
     head = min((int)((16 - ((uintptr_t)p & 15)) & 15) / ES, V);
     nvec = (V - head) / Vec<DT>::N;
+    body = p + head * ES;
   }
   __device__ __forceinline__ int single(int t) const {
     const int j = t < head ? t : t + nvec * Vec<DT>::N;
     return j < V ? j : -1;
   }
-  __device__ __forceinline__ int first(int k) const { return head + k * Vec<DT>::N; }  // element of piece k
   template <bool NT> __device__ __forceinline__ u32x4 load(int k) const {
-    const u32x4* q = (const u32x4*)(p + (int64_t)first(k) * Vec<DT>::ES);
+    const u32x4* q = (const u32x4*)(body + (uint32_t)k * 16u);
     return NT ? __builtin_nontemporal_load(q) : *q;
   }
 };
-// the pieces of a row whose gradient is 16 bytes aligned where the row is, else element by element
+// piece k of the gradient's row: 16 bytes where its rows are aligned as the logits' are, else element by element
 enum { STORE_ELEMENTS, STORE_PLAIN, STORE_STREAM };
-template <int DT> __device__ __forceinline__ void store_piece(char* dz, int j, int how, const float (&x)[Vec<DT>::N]) {
-  u32x4* q = (u32x4*)(dz + (int64_t)j * Vec<DT>::ES);
+template <int DT> __device__ __forceinline__ void store_piece(char* body, int k, int how, const float (&x)[Vec<DT>::N]) {
+  u32x4* q = (u32x4*)(body + (uint32_t)k * 16u);
   if (how == STORE_STREAM) {
     __builtin_nontemporal_store(Vec<DT>::pack(x), q);
     asm volatile("");  // else the compiler makes one plain store of the two
@@ -112,7 +113,7 @@ template <int DT> __device__ __forceinline__ void store_piece(char* dz, int j, i
     *q = Vec<DT>::pack(x);
   } else {
 #pragma unroll
-    for (int e = 0; e < Vec<DT>::N; ++e) put<DT>(dz, j + e, x[e]);
+    for (int e = 0; e < Vec<DT>::N; ++e) put<DT>(q, e, x[e]);
   }
 }
 
@@ -261,8 +262,8 @@ constexpr int LOSS_ALONE = 3;  // a forward without a backward to follow: the lo
 // The backward takes the rows last to first: those that the forward read last are still in the 256 MB cache behind
 // the L2s, and a gradient that does not fit there is stored past it (4096 x 50257 in bf16, forward and backward:
 // 244 us, 233 us with such stores, 214 us in reverse as well).
-template <int DT, int PHASE, int MODE, int T, int NC, int U>
-__global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
+template <int DT, int PHASE, int MODE, int T, int NC, int U, int WPE = 1>
+__global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void loss_row_kernel(LossArgs a) {
   constexpr bool FWD = PHASE == LOSS_FWD || PHASE == LOSS_ALONE, BWD = PHASE == LOSS_BWD, NT = PHASE == LOSS_ALONE;
   __shared__ float red[2][T / 64];
   __shared__ Stat wred[T / 64];
@@ -277,13 +278,14 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
   const char* z = (const char*)a.z + r * a.z_rs * W::ES;
   char* dz = FWD ? nullptr : (char*)a.dz + r * a.dz_rs * W::ES;
   const Row<DT> row(z, V);
+  char* const dbody = FWD ? nullptr : dz + row.head * W::ES;
   const int one = row.single(t);
   const int how = ((uintptr_t)z ^ (uintptr_t)dz) & 15 ? STORE_ELEMENTS : (a.stream ? STORE_STREAM : STORE_PLAIN);
   int64_t y;
   if (!row_label(a, (uint32_t)r, y)) {
     if (!FWD) {
       const float zero[N] = {};
-      for (int k = t; k < row.nvec; k += T) store_piece<DT>(dz, row.first(k), how, zero);
+      for (int k = t; k < row.nvec; k += T) store_piece<DT>(dbody, k, how, zero);
       if (one >= 0) put<DT>(dz, one, 0.f);
     }
     if (t == 0) {
@@ -297,6 +299,11 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
 
   Stat st{-INFINITY, 0.f, 0.f};
   u32x4 held[NC > 0 ? NC : 1];
+  // between two uses of the held row: else the compiler keeps its elements as floats, twice the registers
+  auto keep_packed = [&] {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) asm volatile("" : "+v"(held[c]));
+  };
   if (NC > 0) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -325,6 +332,7 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
       }
     }
     st.m = block_max<T>(mx, red[0]);
+    keep_packed();
     const float x1[1] = {xone};
     add<MODE>(st, x1, lt);
 #pragma unroll
@@ -419,10 +427,11 @@ __global__ __launch_bounds__(T) void loss_row_kernel(LossArgs a) {
     W::unpack(raw, x);
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = dense(x[e]);
-    store_piece<DT>(dz, row.first(k), how, x);
+    store_piece<DT>(dbody, k, how, x);
   };
   if (one >= 0) put<DT>(dz, one, dense(xone));
   if (NC > 0) {
+    keep_packed();
 #pragma unroll
     for (int k = 0; k < NC; ++k)
       if (k * T + t < row.nvec) piece(k * T + t, held[k]);
@@ -505,29 +514,33 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* lo
   if (inv_count) *inv_count = 1.f / (float)n;
 }
 
-template <int DT, int PHASE, int T, int NC, int U> static int run_loss(const LossArgs& a, hipStream_t s) {
+template <int DT, int PHASE, int T, int NC, int U, int WPE = 1> static int run_loss(const LossArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)a.rows), block(T);
   if (a.rows * T > 0xffffffffll) return -2;  // a grid's threads are counted in 32 bits
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, s, a); };
-  if (a.sw == 0.f) go(loss_row_kernel<DT, PHASE, HARD, T, NC, U>);
-  else if (a.hw == 0.f) go(loss_row_kernel<DT, PHASE, SOFT, T, NC, U>);
-  else if (a.T == 1.f) go(loss_row_kernel<DT, PHASE, BOTH_T1, T, NC, U>);
-  else if (a.T == 2.f) go(loss_row_kernel<DT, PHASE, BOTH_T2, T, NC, U>);
-  else go(loss_row_kernel<DT, PHASE, BOTH, T, NC, U>);
+  if (a.sw == 0.f) go(loss_row_kernel<DT, PHASE, HARD, T, NC, U, WPE>);
+  else if (a.hw == 0.f) go(loss_row_kernel<DT, PHASE, SOFT, T, NC, U, WPE>);
+  else if (a.T == 1.f) go(loss_row_kernel<DT, PHASE, BOTH_T1, T, NC, U, WPE>);
+  else if (a.T == 2.f) go(loss_row_kernel<DT, PHASE, BOTH_T2, T, NC, U, WPE>);
+  else go(loss_row_kernel<DT, PHASE, BOTH, T, NC, U, WPE>);
   return hipGetLastError() == hipSuccess ? 0 : -7;
 }
 
-// Threads a row by its pieces: a wave for short rows, more for longer ones; the step the fewest registers that hold the
-// row in a workgroup.
+// Threads a row by its pieces.  The step holds the row in as few registers a thread as the threads allow, with as few
+// rows in flight as keep the memory busy: the bf16 step of 8192 x 32000 takes 201 us with four workgroups of 512
+// threads on a compute unit, 189 us with two of 1024; that of 4096 x 50257 189 us with one workgroup of 1024 threads
+// and 100 registers, 164 us with two in 64 registers (waves a SIMD as the last argument); 4096 x 65536 230 us and, by
+// two of 512 threads, 206 us; 2048 x 130000 244 us held and 257 us read twice.
 template <int DT, int PHASE> static int run_loss(const LossArgs& a, hipStream_t s) {
   const int pieces = a.V / Vec<DT>::N;
   if constexpr (PHASE == LOSS_STEP) {
     if (pieces <= 64 * 4) return run_loss<DT, PHASE, 64, 4, 1>(a, s);
     if (pieces <= 256 * 4) return run_loss<DT, PHASE, 256, 4, 1>(a, s);
     if (pieces <= 512 * 4) return run_loss<DT, PHASE, 512, 4, 1>(a, s);
-    if (pieces <= 512 * 8) return run_loss<DT, PHASE, 512, 8, 1>(a, s);
-    if (pieces <= 1024 * 8) return run_loss<DT, PHASE, 1024, 8, 1>(a, s);
-    if (pieces <= 1024 * 16) return run_loss<DT, PHASE, 1024, 16, 1>(a, s);
+    if (pieces <= 1024 * 4) return run_loss<DT, PHASE, 1024, 4, 1, 8>(a, s);
+    if (pieces <= 1024 * 7) return run_loss<DT, PHASE, 1024, 7, 1, 8>(a, s);
+    if (pieces <= 512 * 16) return run_loss<DT, PHASE, 512, 16, 1, 4>(a, s);
+    if (pieces <= 1024 * 16) return run_loss<DT, PHASE, 1024, 16, 1, 4>(a, s);
     return run_loss<DT, PHASE, 1024, 0, 4>(a, s);
   } else {
     if (pieces <= 64 * 4) return run_loss<DT, PHASE, 64, 0, 4>(a, s);

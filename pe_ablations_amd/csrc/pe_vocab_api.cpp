@@ -94,7 +94,7 @@ int pe_embed_bwd(const void* ids, int32_t id_bytes, int64_t n, const void* dy, i
 
 int pe_loss_check(const pe_loss_params* p) {
   if (!p) return PE_ERR_NULL;
-  if (p->rows < 0 || p->rows > 0x7fffffff || p->vocab <= 0 || p->shift < 0 || p->top_k < 0 || p->top_k > PE_LOSS_MAX_TOP_K)
+  if (p->rows < 0 || p->rows > 0x7fffffff || p->vocab <= 0 || p->vocab > (1 << 28) || p->shift < 0 || p->top_k < 0 || p->top_k > PE_LOSS_MAX_TOP_K)
     return PE_ERR_SHAPE;
   if (p->shift && p->rows % p->shift) return PE_ERR_SHAPE;
   if (!float_dtype(p->dtype) || !id_size(p->label_bytes) || p->reduction < PE_LOSS_NONE || p->reduction > PE_LOSS_MEAN)
