@@ -75,7 +75,8 @@ typedef struct {
 int pe_loss_check(const pe_loss_params* p);
 
 /* Forward: loss (rows floats for PE_LOSS_NONE, else one).  stats (pe_loss_stats_floats floats, or NULL when no
- * backward follows) keeps what pe_loss_bwd needs of each row: the maximum and the two sums. */
+ * backward follows) keeps what pe_loss_bwd needs of each row: the maximum, the two sums, and the teacher's
+ * probabilities, which the backward does not form again (its teacher_ids and teacher_logits are not read). */
 size_t pe_loss_workspace_bytes(const pe_loss_params* p);
 int64_t pe_loss_stats_floats(const pe_loss_params* p);
 int pe_loss_fwd(const pe_loss_params* p, const void* logits, const void* labels, const void* teacher_ids,

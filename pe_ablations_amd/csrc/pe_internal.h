@@ -305,6 +305,8 @@ struct LossArgs {
   int64_t rows; int V, K, reduction;
   float hw, sw, T, factor;
   int stream;             // store the gradient past the caches
+  int32_t* place;         // the teacher's rows: [rows][K + 1] ids and probabilities, [rows][2] sums
+  float *prob, *tsum;
   float* row_loss;        // one per row
   float* stats;           // [rows][3]: maximum, sum, sum at the temperature; [3 rows]: 1 / rows that count
   const float* dloss;     // one, or one per row (PE_LOSS_NONE)
@@ -312,8 +314,9 @@ struct LossArgs {
 };
 enum { LOSS_FWD = 0, LOSS_BWD = 1, LOSS_STEP = 2 };
 int launch_loss(int dtype, int phase, LossArgs a, hipStream_t s);
-// 1 / rows that count (PE_LOSS_MEAN) from the labels
-int launch_loss_count(const LossArgs& a, float* inv_count, hipStream_t s);
+// the teacher's rows, and 1 / rows that count (PE_LOSS_MEAN) from the labels unless inv_count is NULL
+int launch_loss_prepare(const LossArgs& a, float* inv_count, hipStream_t s);
+bool loss_has_teacher(const LossArgs& a);
 // the sum or mean of row_loss; also 1 / rows that count when inv_count is not NULL
 int launch_loss_reduce(const LossArgs& a, float* loss, float* inv_count, hipStream_t s);
 

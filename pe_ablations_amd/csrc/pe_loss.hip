@@ -53,6 +53,10 @@ enum { HARD = 1, SOFT = 2, BOTH = 3, BOTH_T1 = 4, BOTH_T2 = 5 };
 constexpr bool has_hard(int mode) { return mode != SOFT; }
 constexpr bool has_soft(int mode) { return mode != HARD; }
 
+__device__ __forceinline__ float scalar(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
 // 2^x in one instruction; results below 2^-126 are 0
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -189,64 +193,6 @@ template <int T> __device__ __forceinline__ float block_max(float v, float* red)
 
 }  // namespace
 
-// The teacher's pairs of a row, by one wave: the places whose gradient is more than the dense one, that is every
-// different id among the pairs present, with the sum of its probabilities, and the label if it is none of them (y < 0:
-// no label), into `place` / `prob` [K + 1] (-1 where there is none); whether any pair is present, P, and
-// E = sum p ln p.  `tid` and `tp` [K] are the pairs themselves (-1 where absent), which do for the loss (MERGE false).
-template <bool MERGE>
-__device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, float lt, int32_t y, int32_t* tid, float* tp,
-                                            int32_t* place, float* prob, float& P, float& E) {
-  const int lane = threadIdx.x & 63;
-  float mx = -INFINITY;
-  for (int k = lane; k < a.K; k += 64) {
-    const int64_t id = load_id(a.tid, a.tid_bytes, r * a.tid_rs + k);
-    const float x = load_as_float(a.tlog, r * a.tlog_rs + k, a.tlog_dtype);
-    const bool have = id >= 0 && id < a.V && x != -INFINITY;
-    tid[k] = have ? (int32_t)id : -1;
-    tp[k] = x;
-    if (have) mx = fmaxf(mx, x);
-  }
-  mx = wave_max(mx);
-  float n = 0.f;
-  for (int k = lane; k < a.K; k += 64)
-    if (tid[k] >= 0) n += ex2((tp[k] - mx) * lt);
-  n = wave_sum(n);
-  P = n != 0.f ? 1.f : 0.f;
-  const float ln = logf(n);
-  E = 0.f;
-  for (int k = lane; k < a.K; k += 64) {
-    float p = 0.f;
-    if (tid[k] >= 0) {
-      const float d = tp[k] - mx;
-      p = ex2(d * lt) / n;
-      if (p != 0.f) E += p * (d / a.T - ln);
-    }
-    tp[k] = p;
-  }
-  E = wave_sum(E);
-  if (!MERGE) return;
-  bool label = false;  // among the pairs
-  for (int k = lane; k < a.K; k += 64) {
-    const int32_t id = tid[k];
-    float p = 0.f;
-    bool first = id >= 0;
-#pragma unroll 4
-    for (int i = 0; i < a.K; ++i) {
-      const bool same = tid[i] == id;
-      first = first && !(same && i < k);
-      p += same ? tp[i] : 0.f;
-    }
-    place[k] = first ? id : -1;
-    prob[k] = p;
-    label = label || id == y;
-  }
-  label = __ballot(label) != 0;
-  if (lane == 0) {
-    place[a.K] = label ? -1 : y;
-    prob[a.K] = 0.f;
-  }
-}
-
 // gradients beyond this size are stored past the 256 MB cache
 #ifndef STREAMB
 #define STREAMB (128ll << 20)
@@ -267,10 +213,6 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
   constexpr bool FWD = PHASE == LOSS_FWD || PHASE == LOSS_ALONE, BWD = PHASE == LOSS_BWD, NT = PHASE == LOSS_ALONE;
   __shared__ float red[2][T / 64];
   __shared__ Stat wred[T / 64];
-  constexpr int KMAX = has_soft(MODE) ? PE_LOSS_MAX_TOP_K + 1 : 1;
-  __shared__ float tsum[2];  // teacher_row's P and E, and its arrays
-  __shared__ int32_t tid_l[KMAX], place[FWD ? 1 : KMAX];
-  __shared__ float tp_l[KMAX], prob[FWD ? 1 : KMAX];
   using W = Vec<DT>;
   constexpr int N = W::N;
   const int64_t r = BWD ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
@@ -294,10 +236,28 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
     }
     return;
   }
+  y = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(y >> 32)) << 32 |
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)y));
   const bool bad = a.labels && (y < 0 || y >= V);
   const float lt = LOG2E / a.T;
 
   Stat st{-INFINITY, 0.f, 0.f};
+  // The named places, 64 of them or the label's alone, with their logits: fetched by the first wave beside the row and
+  // left in LDS for its use at the end, before a held row's sums, where they made it spill, else behind the row
+  __shared__ int32_t nid[64];
+  __shared__ float np[64], nz[64];
+  const int32_t* place = has_soft(MODE) ? a.place + r * (a.K + 1) : nullptr;
+  const float* prob = has_soft(MODE) ? a.prob + r * (a.K + 1) : nullptr;
+  int32_t id0 = -1;
+  float p0 = 0.f;
+  if (has_soft(MODE)) {
+    if (t < 64 && t <= a.K) {
+      id0 = place[t];
+      p0 = prob[t];
+    }
+  } else if (t == 0 && !bad) {
+    id0 = (int32_t)y;
+  }
   u32x4 held[NC > 0 ? NC : 1];
   // between two uses of the held row: else the compiler keeps its elements as floats, twice the registers
   auto keep_packed = [&] {
@@ -310,14 +270,15 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
       if (c * T + t < row.nvec) held[c] = row.template load<false>(c * T + t);
   }
   const float xone = one >= 0 ? elem<DT>(z, one) : -INFINITY;
-  if (has_soft(MODE) && t >= T - 64) {  // the last wave, which has the fewest pieces; the others need it behind a barrier only
-    float P, E;
-    teacher_row<!FWD>(a, r, lt, has_hard(MODE) && !bad ? (int32_t)y : -1, tid_l, tp_l, place, prob, P, E);
-    if (t == T - 64) {
-      tsum[0] = P;
-      tsum[1] = E;
+  const float z0 = id0 >= 0 ? elem<DT>(z, id0) : 0.f;
+  auto leave_named = [&] {
+    if (t < 64) {
+      nid[t] = id0;
+      np[t] = p0;
+      nz[t] = z0;
     }
-  }
+  };
+  if (NC > 0) leave_named();
   if (BWD) {
     st = Stat{a.stats[3 * r], a.stats[3 * r + 1], a.stats[3 * r + 2]};
   } else if (NC > 0) {
@@ -331,7 +292,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
         for (int e = 0; e < N; ++e) mx = fmaxf(mx, x[e]);
       }
     }
-    st.m = block_max<T>(mx, red[0]);
+    st.m = scalar(block_max<T>(mx, red[0]));
     keep_packed();
     const float x1[1] = {xone};
     add<MODE>(st, x1, lt);
@@ -383,28 +344,40 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
     st = wred[0];
     for (int i = 1; i < T / 64; ++i) st = join<MODE>(st, wred[i], lt);
   }
+  if (!BWD) {  // the same in every thread: scalar registers
+    st.m = scalar(st.m);
+    st.s = scalar(st.s);
+    st.t = scalar(st.t);
+  }
   // without a pair the soft part is 0, which an infinite sum makes of its gradient
-  if (!BWD && has_soft(MODE) && tsum[0] == 0.f) st.t = INFINITY;
-  if (!BWD && t < 64) {  // the first wave: the row's loss
-    float cross = 0.f;   // sum p (m - z) / T
+  if (!BWD && has_soft(MODE) && a.tsum[2 * r] == 0.f) st.t = INFINITY;
+  if (PHASE == LOSS_FWD && t == 0) {
+    a.stats[3 * r] = st.m;
+    a.stats[3 * r + 1] = st.s;
+    a.stats[3 * r + 2] = st.t;
+  }
+  // the row's loss, by the first wave
+  auto row_loss = [&] {
+    float cross = 0.f, zy = nz[0];  // sum p (m - z) / T; the label's logit, of thread 0
     if (has_soft(MODE)) {
-      for (int k = t; k < a.K; k += 64)
-        if (tp_l[k] != 0.f) cross += tp_l[k] * (st.m - elem<DT>(z, tid_l[k]));
+      if (np[t] != 0.f) cross = np[t] * (st.m - nz[t]);
+      for (int k = t + 64; k <= a.K; k += 64)
+        if (prob[k] != 0.f) cross += prob[k] * (st.m - elem<DT>(z, place[k]));
       cross = wave_sum(cross) / a.T;
+      if (has_hard(MODE) && t == 0 && !bad) zy = elem<DT>(z, y);
     }
     if (t == 0) {
       float loss = 0.f;
-      if (has_soft(MODE) && tsum[0] != 0.f) loss = a.sw * a.T * a.T * (tsum[1] + cross + logf(st.t));
-      if (has_hard(MODE) && !bad) loss += a.hw * ((st.m - elem<DT>(z, y)) + logf(st.s));
+      if (has_soft(MODE) && st.t != INFINITY) loss = a.sw * a.T * a.T * (a.tsum[2 * r + 1] + cross + logf(st.t));
+      if (has_hard(MODE) && !bad) loss += a.hw * ((st.m - zy) + logf(st.s));
       a.row_loss[r] = bad ? NAN : loss;
-      if (PHASE == LOSS_FWD) {
-        a.stats[3 * r] = st.m;
-        a.stats[3 * r + 1] = st.s;
-        a.stats[3 * r + 2] = st.t;
-      }
     }
+  };
+  if (NC == 0) leave_named();
+  if (FWD) {
+    if (t < 64) row_loss();
+    return;
   }
-  if (FWD) return;
 
   float c = a.factor;
   if (a.dloss) c *= a.dloss[a.reduction == PE_LOSS_NONE ? r : 0];
@@ -413,6 +386,9 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
   float ch = 0.f, ct = 0.f;
   if (has_hard(MODE)) ch = c * a.hw / st.s;
   if (has_soft(MODE)) ct = c * a.sw * a.T / st.t;
+  c = scalar(c);
+  ch = scalar(ch);
+  ct = scalar(ct);
   auto dense = [&](float x) {
     float e, et;
     exps<MODE>(x - st.m, lt, e, et);
@@ -447,39 +423,40 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
     for (; k < row.nvec; k += T) piece(k, row.template load<false>(k));
   }
   __syncthreads();
+  if (t >= 64) return;
   // the named places again
-  if (has_soft(MODE)) {
-    for (int k = t; k <= a.K; k += T) {
-      const int32_t id = place[k];
-      if (id < 0) continue;
-      float g = dense(elem<DT>(z, id)) - c * a.sw * a.T * prob[k];
-      if (has_hard(MODE) && id == y) g -= c * a.hw;
-      put<DT>(dz, id, g);
-    }
-  } else if (t == 0 && !bad) {
-    put<DT>(dz, y, dense(elem<DT>(z, y)) - c * a.hw);
-  }
+  auto named = [&](int32_t id, float x, float p) {
+    if (id < 0) return;
+    float g = dense(x);
+    if (has_soft(MODE)) g -= c * a.sw * a.T * p;
+    if (has_hard(MODE) && id == y) g -= c * a.hw;
+    put<DT>(dz, id, g);
+  };
+  named(nid[t], nz[t], np[t]);
+  if (has_soft(MODE))
+    for (int k = t + 64; k <= a.K; k += 64)
+      if (place[k] >= 0) named(place[k], elem<DT>(z, place[k]), prob[k]);
+  if (!BWD) row_loss();
 }
 
-// 1 / rows that count, and the sum or mean of the row losses: one workgroup, thread t taking rows t, t + 1024, ...
-template <bool SUM>
-__global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* loss, float* inv_count) {
-  __shared__ double rs[16];
-  __shared__ int32_t rn[16];
+// 1 / rows that count, and the sum or mean of the row losses (SUM), by one workgroup of T threads, thread t taking rows
+// t, t + T, ..., the loads of U rows in flight.
+template <bool SUM, int T> __device__ __forceinline__ void reduce_rows(const LossArgs& a, float* loss, float* inv_count) {
+  __shared__ double rs[T / 64];
+  __shared__ int32_t rn[T / 64];
   const int t = threadIdx.x;
   double s = 0.;
   int32_t n = 0;
-  // without a branch between the loads: U rows' in flight
   const uint32_t rows = (uint32_t)a.rows, w = (uint32_t)a.label_bytes / 4, shift = (uint32_t)a.shift;
   const int32_t* lab = (const int32_t*)a.labels;
   constexpr int U = 8;
-  for (uint32_t r0 = t; r0 < rows; r0 += U * 1024) {
+  for (uint32_t r0 = t; r0 < rows; r0 += U * T) {
     float x[U];
     int32_t lo[U], hi[U];
     bool last[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t r = min(r0 + u * 1024, rows - 1);
+      const uint32_t r = min(r0 + u * T, rows - 1);
       x[u] = SUM ? a.row_loss[r] : 0.f;
       last[u] = shift && (r + 1) % shift == 0;
       const uint64_t i = (uint64_t)(shift && !last[u] ? r + 1 : r) * w;
@@ -489,7 +466,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* lo
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t y = w == 2 ? (int64_t)((uint64_t)(uint32_t)hi[u] << 32 | (uint32_t)lo[u]) : (int64_t)lo[u];
-      if (r0 + u * 1024 < rows) {
+      if (r0 + u * T < rows) {
         s += x[u];
         n += !lab || (!last[u] && y != a.ignore) ? 1 : 0;
       }
@@ -506,12 +483,108 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* lo
   }
   __syncthreads();
   if (t != 0) return;
-  for (int i = 1; i < 16; ++i) {
+  for (int i = 1; i < T / 64; ++i) {
     s += rs[i];
     n += rn[i];
   }
   if (SUM) *loss = (float)(a.reduction == PE_LOSS_MEAN ? s / (double)n : s);
   if (inv_count) *inv_count = 1.f / (float)n;
+}
+
+__global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* loss, float* inv_count) {
+  reduce_rows<true, 1024>(a, loss, inv_count);
+}
+__global__ __launch_bounds__(1024) void loss_count_kernel(LossArgs a, float* inv_count) {
+  reduce_rows<false, 1024>(a, nullptr, inv_count);
+}
+
+// The teacher's pairs, ahead of the rows' workgroups, which would wait for them: a wave takes a row.  What the rows need
+// of them (LossArgs::place, prob, tsum) is the places whose gradient is more than the dense one, that is every
+// different id among the pairs present with the sum of its probabilities and behind them the label if it is none of
+// them (-1 where there is none); whether any pair is present, P; and E = sum p ln p.
+constexpr int TEACHER_ROWS = 4;
+constexpr int teacher_pitch(int K) { return (K + 3) / 4 * 4; }
+
+__device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, int32_t* tid, float* tp) {
+  const int lane = threadIdx.x & 63, K = a.K, pitch = teacher_pitch(K);
+  int64_t y;
+  if (!row_label(a, (uint32_t)r, y)) return;
+  if (!a.labels || a.hw == 0.f || y < 0 || y >= a.V) y = -1;
+  const float lt = LOG2E / a.T;
+  float mx = -INFINITY;
+  for (int k = lane; k < pitch; k += 64) {
+    int64_t id = -1;
+    float x = 0.f;
+    if (k < K) {
+      id = load_id(a.tid, a.tid_bytes, r * a.tid_rs + k);
+      x = load_as_float(a.tlog, r * a.tlog_rs + k, a.tlog_dtype);
+    }
+    const bool have = id >= 0 && id < a.V && x != -INFINITY;
+    tid[k] = have ? (int32_t)id : -1;
+    tp[k] = x;
+    if (have) mx = fmaxf(mx, x);
+  }
+  mx = wave_max(mx);
+  float n = 0.f;
+  for (int k = lane; k < K; k += 64)
+    if (tid[k] >= 0) n += ex2((tp[k] - mx) * lt);
+  n = wave_sum(n);
+  const float ln = logf(n);
+  float E = 0.f;
+  for (int k = lane; k < K; k += 64) {
+    float p = 0.f;
+    if (tid[k] >= 0) {
+      const float d = tp[k] - mx;
+      p = ex2(d * lt) / n;
+      if (p != 0.f) E += p * (d / a.T - ln);
+    }
+    tp[k] = p;
+  }
+  E = wave_sum(E);
+  bool label = false;  // among the pairs
+  int32_t* place = a.place + r * (K + 1);
+  float* prob = a.prob + r * (K + 1);
+  for (int k = lane; k < (K + 63) / 64 * 64; k += 64) {
+    const int32_t id = k < K ? tid[k] : -1;
+    bool first = id >= 0;
+    int same = 0;
+    for (int i = 0; i < pitch; i += 4) {
+      const int4 o = *(const int4*)(tid + i);
+      const bool s0 = o.x == id, s1 = o.y == id, s2 = o.z == id, s3 = o.w == id;
+      same += (int)s0 + (int)s1 + (int)s2 + (int)s3;
+      first = first && !((s0 && i < k) || (s1 && i + 1 < k) || (s2 && i + 2 < k) || (s3 && i + 3 < k));
+    }
+    float p = k < K ? tp[k] : 0.f;
+    if (first && same > 1) {  // an id that comes twice
+      p = 0.f;
+      for (int i = 0; i < K; ++i) p += tid[i] == id ? tp[i] : 0.f;
+    }
+    if (k < K) {
+      place[k] = first ? id : -1;
+      prob[k] = first ? p : 0.f;
+    }
+    label = label || (id >= 0 && id == y);
+  }
+  label = __ballot(label) != 0;
+  if (lane == 0) {
+    place[K] = label ? -1 : (int32_t)y;
+    prob[K] = 0.f;
+    a.tsum[2 * r] = n != 0.f ? 1.f : 0.f;
+    a.tsum[2 * r + 1] = E;
+  }
+}
+
+// the teacher's rows; with inv_count also the number of rows that count, by a workgroup ahead of them
+__global__ __launch_bounds__(TEACHER_ROWS * 64) void loss_teacher_kernel(LossArgs a, float* inv_count) {
+  extern __shared__ __attribute__((aligned(16))) char dyn[];
+  int64_t block = blockIdx.x;
+  if (inv_count && block-- == 0) {
+    reduce_rows<false, TEACHER_ROWS * 64>(a, nullptr, inv_count);
+    return;
+  }
+  const int w = threadIdx.x >> 6, pitch = teacher_pitch(a.K);
+  const int64_t r = block * TEACHER_ROWS + w;
+  if (r < a.rows) teacher_row(a, r, (int32_t*)dyn + 2 * w * pitch, (float*)dyn + (2 * w + 1) * pitch);
 }
 
 template <int DT, int PHASE, int T, int NC, int U, int WPE = 1> static int run_loss(const LossArgs& a, hipStream_t s) {
@@ -538,7 +611,7 @@ template <int DT, int PHASE> static int run_loss(const LossArgs& a, hipStream_t 
     if (pieces <= 256 * 4) return run_loss<DT, PHASE, 256, 4, 1>(a, s);
     if (pieces <= 512 * 4) return run_loss<DT, PHASE, 512, 4, 1>(a, s);
     if (pieces <= 1024 * 4) return run_loss<DT, PHASE, 1024, 4, 1, 8>(a, s);
-    if (pieces <= 1024 * 7) return run_loss<DT, PHASE, 1024, 7, 1, 8>(a, s);
+    if (pieces <= 1024 * 7 && a.sw == 0.f) return run_loss<DT, PHASE, 1024, 7, 1, 8>(a, s);
     if (pieces <= 512 * 16) return run_loss<DT, PHASE, 512, 16, 1, 4>(a, s);
     if (pieces <= 1024 * 16) return run_loss<DT, PHASE, 1024, 16, 1, 4>(a, s);
     return run_loss<DT, PHASE, 1024, 0, 4>(a, s);
@@ -564,13 +637,21 @@ int launch_loss(int dtype, int phase, LossArgs a, hipStream_t s) {
   return loss_phase<2>(phase, a, s);
 }
 
-int launch_loss_count(const LossArgs& a, float* inv_count, hipStream_t s) {
-  hipLaunchKernelGGL(loss_reduce_kernel<false>, dim3(1), dim3(1024), 0, s, a, (float*)nullptr, inv_count);
+bool loss_has_teacher(const LossArgs& a) { return a.sw != 0.f; }
+
+int launch_loss_prepare(const LossArgs& a, float* inv_count, hipStream_t s) {
+  if (a.rows > 0 && loss_has_teacher(a)) {
+    const unsigned blocks = (unsigned)((a.rows + TEACHER_ROWS - 1) / TEACHER_ROWS) + (inv_count ? 1 : 0);
+    hipLaunchKernelGGL(loss_teacher_kernel, dim3(blocks), dim3(TEACHER_ROWS * 64), 8 * TEACHER_ROWS * teacher_pitch(a.K), s, a,
+                       inv_count);
+  } else if (inv_count) {
+    hipLaunchKernelGGL(loss_count_kernel, dim3(1), dim3(1024), 0, s, a, inv_count);
+  }
   return hipGetLastError() == hipSuccess ? 0 : -7;
 }
 
 int launch_loss_reduce(const LossArgs& a, float* loss, float* inv_count, hipStream_t s) {
-  hipLaunchKernelGGL(loss_reduce_kernel<true>, dim3(1), dim3(1024), 0, s, a, loss, inv_count);
+  hipLaunchKernelGGL(loss_reduce_kernel, dim3(1), dim3(1024), 0, s, a, loss, inv_count);
   return hipGetLastError() == hipSuccess ? 0 : -7;
 }
 

@@ -22,8 +22,13 @@ int embed_check(const void* ids, int32_t id_bytes, int64_t n, const void* x, int
   return PE_OK;
 }
 
-// the row losses, and one float behind them for 1 / rows that count
-int64_t loss_ws_floats(const pe_loss_params* p) { return p->rows + 1; }
+// the teacher's rows: ids and probabilities of K + 1 places, two sums
+int64_t teacher_floats(const pe_loss_params* p) { return p->soft_weight > 0.f ? p->rows * (2 * (int64_t)p->top_k + 4) : 0; }
+void set_teacher(pe::LossArgs& a, float* at) {
+  a.place = (int32_t*)at;
+  a.prob = at + a.rows * (a.K + 1);
+  a.tsum = a.prob + a.rows * (a.K + 1);
+}
 
 pe::LossArgs loss_args(const pe_loss_params* p, const void* z, const void* labels, const void* tid, const void* tlog) {
   pe::LossArgs a;
@@ -110,10 +115,11 @@ int pe_loss_check(const pe_loss_params* p) {
 }
 
 size_t pe_loss_workspace_bytes(const pe_loss_params* p) {
-  return pe_loss_check(p) ? 0 : (size_t)loss_ws_floats(p) * 4;
+  // the row losses, 1 / rows that count, the teacher's rows
+  return pe_loss_check(p) ? 0 : (size_t)(p->rows + 1 + teacher_floats(p)) * 4;
 }
 
-int64_t pe_loss_stats_floats(const pe_loss_params* p) { return pe_loss_check(p) ? 0 : 3 * p->rows + 1; }
+int64_t pe_loss_stats_floats(const pe_loss_params* p) { return pe_loss_check(p) ? 0 : 3 * p->rows + 1 + teacher_floats(p); }
 
 int pe_loss_fwd(const pe_loss_params* p, const void* logits, const void* labels, const void* teacher_ids,
                 const void* teacher_logits, float* loss, float* stats, void* workspace, size_t ws_bytes, void* stream) {
@@ -127,6 +133,8 @@ int pe_loss_fwd(const pe_loss_params* p, const void* logits, const void* labels,
   const bool whole = p->reduction != PE_LOSS_NONE;
   a.row_loss = whole ? (float*)workspace : loss;
   a.stats = stats;
+  set_teacher(a, stats ? stats + 3 * p->rows + 1 : (float*)workspace + p->rows + 1);
+  if ((rc = pe::launch_loss_prepare(a, nullptr, (hipStream_t)stream))) return rc;
   if ((rc = pe::launch_loss(p->dtype, pe::LOSS_FWD, a, (hipStream_t)stream)) || !whole) return rc;
   return pe::launch_loss_reduce(a, loss, stats ? stats + 3 * p->rows : nullptr, (hipStream_t)stream);
 }
@@ -142,6 +150,7 @@ int pe_loss_bwd(const pe_loss_params* p, const void* logits, const void* labels,
   pe::LossArgs a = loss_args(p, logits, labels, teacher_ids, teacher_logits);
   a.dz = dlogits;
   a.stats = const_cast<float*>(stats);
+  set_teacher(a, a.stats + 3 * p->rows + 1);
   a.dloss = dloss;
   a.inv_count = p->reduction == PE_LOSS_MEAN ? stats + 3 * p->rows : nullptr;
   return pe::launch_loss(p->dtype, pe::LOSS_BWD, a, (hipStream_t)stream);
@@ -161,11 +170,10 @@ int pe_loss_step(const pe_loss_params* p, const void* logits, const void* labels
   a.dz = dlogits;
   a.row_loss = (float*)workspace;
   a.dloss = grad_scale;
-  if (p->reduction == PE_LOSS_MEAN) {
-    float* inv = (float*)workspace + p->rows;
-    if ((rc = pe::launch_loss_count(a, inv, (hipStream_t)stream))) return rc;
-    a.inv_count = inv;
-  }
+  set_teacher(a, (float*)workspace + p->rows + 1);
+  float* inv = p->reduction == PE_LOSS_MEAN ? (float*)workspace + p->rows : nullptr;
+  if ((rc = pe::launch_loss_prepare(a, inv, (hipStream_t)stream))) return rc;
+  a.inv_count = inv;
   if ((rc = pe::launch_loss(p->dtype, pe::LOSS_STEP, a, (hipStream_t)stream))) return rc;
   return pe::launch_loss_reduce(a, loss, nullptr, (hipStream_t)stream);
 }

@@ -100,12 +100,14 @@ def _forward(p, x, labels, tid, tlog, keep):
     L, dev = _lib.lib(), x.device
     whole = p.reduction != _lib.PE_LOSS_NONE
     loss = torch.empty((1,) if whole else (p.rows,), dtype=torch.float32, device=dev)
+    ref = ctypes.byref(p)
     # one buffer: the statistics, then the workspace
-    n = 3 * p.rows + 1 if keep else 0
-    buf = torch.empty(n + p.rows + 1, dtype=torch.float32, device=dev)
+    n = L.pe_loss_stats_floats(ref) if keep else 0
+    nb = L.pe_loss_workspace_bytes(ref)
+    buf = torch.empty(n + nb // 4, dtype=torch.float32, device=dev)
     with _on(dev):
-        rc = L.pe_loss_fwd(ctypes.byref(p), x.data_ptr(), _ptr(labels), _ptr(tid), _ptr(tlog), loss.data_ptr(),
-                           buf.data_ptr() if keep else None, buf.data_ptr() + 4 * n, 4 * (p.rows + 1), _stream(dev))
+        rc = L.pe_loss_fwd(ref, x.data_ptr(), _ptr(labels), _ptr(tid), _ptr(tlog), loss.data_ptr(),
+                           buf.data_ptr() if keep else None, buf.data_ptr() + 4 * n, nb, _stream(dev))
     _lib.check(rc)
     return loss, buf
 
@@ -231,10 +233,13 @@ def loss_and_grad(logits: torch.Tensor, labels: Optional[torch.Tensor], *, teach
             raise ValueError(f"loss_and_grad: grad_scale must be a number or one fp32 element on {dev}")
     else:
         p.grad_factor = float(grad_scale)
-    out = torch.empty(p.rows + 2, dtype=torch.float32, device=dev)  # the loss, then the workspace
+    L, ref = _lib.lib(), ctypes.byref(p)
+    nb = L.pe_loss_workspace_bytes(ref)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     dz = torch.empty((p.rows, p.vocab), dtype=x.dtype, device=dev)
     with _on(dev):
-        rc = _lib.lib().pe_loss_step(ctypes.byref(p), x.data_ptr(), _ptr(lab), _ptr(tid), _ptr(tlog), _ptr(scale),
-                                     out.data_ptr(), dz.data_ptr(), out.data_ptr() + 4, 4 * (p.rows + 1), _stream(dev))
+        rc = L.pe_loss_step(ref, x.data_ptr(), _ptr(lab), _ptr(tid), _ptr(tlog), _ptr(scale), loss.data_ptr(),
+                            dz.data_ptr(), ws.data_ptr(), nb, _stream(dev))
     _lib.check(rc)
-    return out[0], dz.view(logits.shape)
+    return loss, dz.view(logits.shape)

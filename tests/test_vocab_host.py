@@ -72,7 +72,8 @@ def test_loss_check(lib, over, code):
     p = params(**over)
     assert lib.pe_loss_check(ctypes.byref(p)) == E[code]
     good = code == "PE_OK"
-    assert lib.pe_loss_stats_floats(ctypes.byref(p)) == (3 * p.rows + 1 if good else 0)
+    teacher = p.rows * (2 * p.top_k + 4) if p.soft_weight > 0 else 0
+    assert lib.pe_loss_stats_floats(ctypes.byref(p)) == (3 * p.rows + 1 + teacher if good else 0)
     nb = lib.pe_loss_workspace_bytes(ctypes.byref(p))
     assert nb >= 4 * (p.rows + 1) if good else nb == 0
 
