@@ -193,11 +193,10 @@ template <int T> __device__ __forceinline__ float block_max(float v, float* red)
 
 }  // namespace
 
-// gradients beyond this size are stored past the 256 MB cache
-#ifndef STREAMB
-#define STREAMB (128ll << 20)
-#endif
-constexpr int64_t STREAM_BYTES = STREAMB;
+// Gradients beyond this size are stored past the 256 MB cache, smaller ones are left in it for the products that read
+// them next (step, then both products of the output projection, hidden 512, vocabulary 32000: 62 MB 269 us streamed and
+// 261 us not, 125 MB 424 and 432 us, 250 MB 695 and 704 us).
+constexpr int64_t STREAM_BYTES = 96ll << 20;
 
 constexpr int LOSS_ALONE = 3;  // a forward without a backward to follow: the logits are read past the caches
 

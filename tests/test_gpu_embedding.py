@@ -99,6 +99,22 @@ def test_gradient_many_tokens(cuda, n):
     check_grad(embedding_backward(ids, dy, 70001), ids, dy, 70001, 1.0, "fp32")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,V,H,kind", [
+    (4096, 16384, 1030, "zipf"), (4096, 16383, 1030, "zipf"),  # where the lanes on a row change, several slices
+    (4096, 700, 264, "one"), (4097, 700, 264, "one"),          # one launch and a sort, a long run
+    (4096, 64, 8, "two"), (4097, 1, 40, "one"), (5000, 2, 8, "two"),
+    (4200, 1 << 20, 4, "uniform"), (4200, (1 << 20) + 3, 2, "uniform"), (700, 3_000_001, 1, "zipf"),  # digits of the sort
+    (65536, 900, 16, "zipf"), (65537, 900, 16, "zipf"), (66000, 5, 8, "one"),  # tiles and chunks of the sort
+])
+def test_gradient_borders(cuda, n, V, H, kind, dtype):
+    """Sizes on either side of the kernels' borders."""
+    ids, _, dy = make(cuda, n, V, H, dtype, kind=kind)
+    if kind == "uniform":
+        ids[::7], ids[3] = V - 1, 0
+    check_grad(embedding_backward(ids, dy, V, scale=-0.5), ids, dy, V, -0.5, dtype)
+
+
 def test_gradient_padding_and_outside(cuda):
     ids, _, dy = make(cuda, 3000, 100, 24, "fp32")
     ids[::2] = 7
