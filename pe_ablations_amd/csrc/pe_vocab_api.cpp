@@ -127,6 +127,7 @@ int pe_loss_fwd(const pe_loss_params* p, const void* logits, const void* labels,
   if (rc) return rc;
   if (p->rows == 0 && p->reduction == PE_LOSS_NONE) return PE_OK;
   if (!loss) return PE_ERR_NULL;
+  if (!aligned(loss, 4) || !aligned(stats, 4)) return PE_ERR_STRIDE;
   if (!workspace || !aligned(workspace, 4) || ws_bytes < pe_loss_workspace_bytes(p)) return PE_ERR_WORKSPACE;
   if ((rc = pe::device_ready())) return rc;
   pe::LossArgs a = loss_args(p, logits, labels, teacher_ids, teacher_logits);
@@ -145,7 +146,7 @@ int pe_loss_bwd(const pe_loss_params* p, const void* logits, const void* labels,
   if (rc) return rc;
   if (p->rows == 0) return PE_OK;
   if (!stats || !dloss || !dlogits) return PE_ERR_NULL;
-  if (!aligned(dlogits, elem_size(p->dtype))) return PE_ERR_STRIDE;
+  if (!aligned(dlogits, elem_size(p->dtype)) || !aligned(stats, 4) || !aligned(dloss, 4)) return PE_ERR_STRIDE;
   if ((rc = pe::device_ready())) return rc;
   pe::LossArgs a = loss_args(p, logits, labels, teacher_ids, teacher_logits);
   a.dz = dlogits;
@@ -163,7 +164,7 @@ int pe_loss_step(const pe_loss_params* p, const void* logits, const void* labels
   if (rc) return rc;
   if (p->reduction == PE_LOSS_NONE) return PE_ERR_MODE;
   if (!loss || (p->rows && !dlogits)) return PE_ERR_NULL;
-  if (!aligned(dlogits, elem_size(p->dtype))) return PE_ERR_STRIDE;
+  if (!aligned(dlogits, elem_size(p->dtype)) || !aligned(loss, 4) || !aligned(grad_scale, 4)) return PE_ERR_STRIDE;
   if (!workspace || !aligned(workspace, 4) || ws_bytes < pe_loss_workspace_bytes(p)) return PE_ERR_WORKSPACE;
   if ((rc = pe::device_ready())) return rc;
   pe::LossArgs a = loss_args(p, logits, labels, teacher_ids, teacher_logits);

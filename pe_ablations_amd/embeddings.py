@@ -11,7 +11,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .functional import _dtype_code, _expression_grads, _on, _ptr, _stream, plain_autograd
+from .functional import _dtype_code, _on, _ptr, _stream, plain_autograd
 
 _FLOATS = (torch.bfloat16, torch.float32, torch.float16)
 _INTS = (torch.int64, torch.int32)
@@ -93,23 +93,31 @@ def embedding_backward(ids: torch.Tensor, dy: torch.Tensor, vocab_size: int, *, 
     return _gradient(ids, dy, vocab_size, float(scale), pad)
 
 
+def _gradient_expression(ids: torch.Tensor, dy: torch.Tensor, V: int, scale: float, pad: int) -> torch.Tensor:
+    """_gradient in torch operations, which higher derivatives differentiate (it is linear in dy)."""
+    ids = ids.reshape(-1).long()
+    keep = (ids >= 0) & (ids < V) & (ids != pad)
+    rows = torch.where(keep[:, None], dy.reshape(ids.numel(), dy.shape[-1]).float(), 0.0)
+    dw = torch.zeros((V, dy.shape[-1]), device=dy.device).index_add(0, torch.where(keep, ids, 0), rows)
+    return (dw * scale).to(dy.dtype)
+
+
 class EmbeddingFn(torch.autograd.Function):
-    """The lookup with pe_embed_bwd as its backward; under create_graph and with batched gradients the
-    backward differentiates F.embedding(ids, weight) * scale (as RMSNormFn)."""
+    """The lookup with pe_embed_bwd as its backward.  It keeps the ids alone, as F.embedding does: the weight may be
+    changed in place before the backward.  Under create_graph and with batched gradients the backward is the
+    gradient in torch operations."""
 
     @staticmethod
     def forward(ctx, weight, ids, scale, pad):
-        ctx.save_for_backward(weight, ids)
-        ctx.scale, ctx.pad = scale, pad
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.pad = weight.shape[0], scale, pad
         return _lookup(ids, weight, scale)
 
     @staticmethod
     def backward(ctx, dy):
-        weight, ids = ctx.saved_tensors
-        if torch.is_grad_enabled() or not plain_autograd(dy):
-            return _expression_grads(lambda: F.embedding(ids, weight, None if ctx.pad < 0 else ctx.pad) * ctx.scale,
-                                     (weight,), ctx, dy) + (None, None, None)
-        return _gradient(ids, dy, weight.shape[0], ctx.scale, ctx.pad), None, None, None
+        (ids,) = ctx.saved_tensors
+        fn = _gradient if plain_autograd(dy) and not torch.is_grad_enabled() else _gradient_expression
+        return fn(ids, dy, ctx.rows, ctx.scale, ctx.pad), None, None, None
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
@@ -117,8 +125,11 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     """weight[ids] * scale, (*ids.shape, dim) in the weight's dtype, the product in fp32 and rounded once.
     weight (vocab, dim) bf16 / fp16 / fp32 on the GPU, ids int64 / int32 on the same device.  Differentiable in
     the weight (embedding_backward); the rows of padding_idx get no gradient.  An id outside the vocabulary
-    cannot be refused without waiting for the GPU: its row is NaN."""
+    cannot be refused without waiting for the GPU: its row is NaN.  Where something other than plain autograd looks
+    at the weight (functorch, forward mode, tracing, compiling) it is F.embedding(ids, weight) * scale."""
     pad = _check(ids, weight, padding_idx)
+    if not plain_autograd(weight):
+        return F.embedding(ids, weight, None if pad < 0 else pad) * scale
     if weight.requires_grad and torch.is_grad_enabled():
         if ids.numel() > _MAX_TOKENS:
             raise ValueError(f"embedding: {ids.numel()} tokens in one call with gradients, at most {_MAX_TOKENS}")

@@ -17,7 +17,9 @@ labels (..., S) of the same positions and holds row s to label s + 1, without th
 slicing would make; the last row of each sequence does not count.
 
 Everything is computed in fp32 from bf16, fp16 or fp32 logits, losses are fp32, gradients are rounded once to the
-logits' dtype; sums run in a fixed order.  A label that is neither in the vocabulary nor ignore_index, which
+logits' dtype; sums run in a fixed order.  The differentiable forms keep the logits for their backward, so these must
+not be changed in place in between (autograd notices).  Where something other than plain autograd looks at the logits
+(functorch, forward mode, tracing, compiling) the losses are the same expressions in torch operations.  A label that is neither in the vocabulary nor ignore_index, which
 cannot be refused without waiting for the GPU, makes its row's loss and gradient NaN.
 """
 
@@ -178,6 +180,8 @@ class LossFn(torch.autograd.Function):
 
 def _loss(what, logits, labels, teacher_ids, teacher_logits, temperature, soft_weight, ignore_index, reduction, shift):
     args = (float(temperature), float(soft_weight), int(ignore_index), reduction, bool(shift))
+    if logits.is_cuda and not plain_autograd(logits):
+        return _expression(logits, labels, teacher_ids, teacher_logits, *args)
     prepared = _prepare(what, logits, labels, teacher_ids, teacher_logits, *args)
     if torch.is_grad_enabled() and logits.requires_grad:
         return LossFn.apply(logits, labels, teacher_ids, teacher_logits, args, prepared)

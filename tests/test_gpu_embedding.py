@@ -183,6 +183,47 @@ def test_higher_derivatives_and_batched_gradients(cuda):
     assert gb.shape == (24, 6, 8) and float(gb.sum()) == 48.0
 
 
+def test_transforms_of_torch(cuda):
+    """functorch and forward mode see F.embedding's expression."""
+    w = torch.randn(9, 8, device=cuda)
+    ids = torch.tensor([1, 8, 1], device=cuda)
+    f = lambda x: (embedding(ids, x, scale=2.0, padding_idx=8) ** 2).sum()  # noqa: E731
+    want = torch.zeros_like(w)
+    want[1] = 2 * 8 * w[1]
+    assert torch.allclose(torch.func.grad(f)(w), want, rtol=1e-5, atol=1e-5)
+    ws = torch.stack([w, w * 2])
+    assert torch.allclose(torch.func.vmap(lambda x: embedding(ids, x, scale=2.0))(ws), 2.0 * ws[:, ids])
+    out, tangent = torch.func.jvp(lambda x: embedding(ids, x, scale=2.0), (w,), (torch.ones_like(w),))
+    assert torch.equal(out, 2 * w[ids]) and bool((tangent == 2).all())
+
+
+def test_weight_changed_before_the_backward(cuda):
+    """As with F.embedding, whose backward needs the ids alone."""
+    w = torch.randn(9, 8, device=cuda, requires_grad=True)
+    ids = torch.tensor([1, 8, 1], device=cuda)
+    out = embedding(ids, w)
+    with torch.no_grad():
+        w.mul_(2)
+    out.sum().backward()
+    assert w.grad[1, 0] == 2 and w.grad[8, 3] == 1 and w.grad[0, 0] == 0
+
+
+def test_past_32_bit_offsets(cuda):
+    """A table and gradients of over 2^32 bytes and 2^31 elements."""
+    V, H, n = 70001, 32768, 66000
+    w = torch.zeros(V, H, dtype=torch.bfloat16, device=cuda)
+    w[V - 1], w[V - 2], w[3] = 3.0, 2.0, 1.0
+    out = embedding(torch.tensor([V - 1, 3, V - 2, 0], device=cuda), w, scale=2.0)
+    assert out.float().mean(-1).tolist() == [6.0, 2.0, 4.0, 0.0]
+    ids = torch.arange(n, device=cuda) % 5000 + (V - 5000)
+    dy = w[:n]
+    dy[n - 1] = 1.0
+    dw = embedding_backward(ids, dy, V)
+    rows = dw.float().sum(-1)
+    want = torch.zeros(V, device=cuda).index_add_(0, ids, dy.float().mean(-1) * H)
+    assert torch.equal(rows, want) and int((rows != 0).sum()) == 2
+
+
 def test_module(cuda):
     m = TokenEmbedding(64, 32, scale=4.0).to(cuda)
     ids = torch.randint(0, 64, (2, 9), device=cuda)

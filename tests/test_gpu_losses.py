@@ -304,6 +304,35 @@ def test_higher_derivatives_and_batched_gradients(cuda):
     assert gb.shape == (3, 3, 20) and bool((gb[1] == 0).all())
 
 
+def test_transforms_of_torch(cuda):
+    z, y, tid, tlog = make(cuda, 4, 30, "fp32", 5)
+    kw = dict(temperature=2.0, reduction="sum")
+    _, want = loss_and_grad(z, y, teacher_ids=tid, teacher_logits=tlog, **kw)
+    got = torch.func.grad(lambda x: distillation_loss(x, y, tid, tlog, **kw))(z)
+    assert torch.allclose(got, want, atol=1e-6)
+    loss, tangent = torch.func.jvp(lambda x: cross_entropy(x, y, reduction="none"), (z,), (torch.ones_like(z),))
+    assert torch.allclose(loss, cross_entropy(z, y, reduction="none"), atol=1e-5) and bool((tangent.abs() < 1e-5).all())
+
+
+def test_past_32_bit_offsets(cuda):
+    """Logits and a gradient of over 2^32 bytes and 2^31 elements: the last rows are those of the rows alone."""
+    N, V = 44000, 50257
+    z = torch.zeros(N, V, dtype=torch.bfloat16, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    z[-3:] = torch.randn(3, V, generator=g, device=cuda).bfloat16() * 3
+    y = torch.full((N,), -100, device=cuda)
+    y[-3:], y[0] = torch.tensor([5, 50256, 777], device=cuda), 1
+    rows = cross_entropy(z, y, reduction="none")
+    assert torch.equal(rows[-3:], cross_entropy(z[-3:], y[-3:], reduction="none")) and bool((rows[1:-3] == 0).all())
+    _, dz = loss_and_grad(z, y, reduction="sum")
+    _, alone = loss_and_grad(z[-3:], y[-3:], reduction="sum")
+    assert torch.equal(dz[-3:], alone) and not bool(dz[1:-3].any())
+    del dz
+    x = z.requires_grad_(True)
+    (dz,) = torch.autograd.grad(cross_entropy(x, y, reduction="sum"), x)
+    assert off_by(dz[-3:], alone, 2.0 ** -8 * alone.double().abs() + 1e-30) <= 0 and not bool(dz[1:-3].any())
+
+
 def test_leaf_changed_before_the_backward_is_noticed(cuda):
     z = torch.randn(3, 20, device=cuda, requires_grad=True)
     x = z * 1
