@@ -329,6 +329,7 @@ struct EmbedArgs {
   int32_t *key, *order;         // the tokens sorted by id: their ids and positions
   int2* run;                    // each id's first sorted token and the one behind its last
   float* part; int chunk;       // sums over chunks of sorted tokens
+  int stream;                   // store y past the caches
   int pieces, lpr, slices;      // vector accesses a row, lanes that work on one, and its column slices
 };
 int launch_embed_fwd(int dtype, EmbedArgs a, hipStream_t s);

@@ -111,8 +111,10 @@ enum { STORE_ELEMENTS, STORE_PLAIN, STORE_STREAM };
 template <int DT> __device__ __forceinline__ void store_piece(char* body, int k, int how, const float (&x)[Vec<DT>::N]) {
   u32x4* q = (u32x4*)(body + (uint32_t)k * 16u);
   if (how == STORE_STREAM) {
-    __builtin_nontemporal_store(Vec<DT>::pack(x), q);
-    asm volatile("");  // else the compiler makes one plain store of the two
+    const u32x4 r = Vec<DT>::pack(x);
+    asm volatile("");  // on either side: else the compiler makes one plain store of the two
+    __builtin_nontemporal_store(r, q);
+    asm volatile("");
   } else if (how == STORE_PLAIN) {
     *q = Vec<DT>::pack(x);
   } else {
