@@ -506,6 +506,13 @@ __global__ __launch_bounds__(1024) void loss_count_kernel(LossArgs a, float* inv
 constexpr int TEACHER_ROWS = 4;
 constexpr int teacher_pitch(int K) { return (K + 3) / 4 * 4; }
 
+// what the wave's lanes wrote to LDS is there for the others
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 __device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, int32_t* tid, float* tp) {
   const int lane = threadIdx.x & 63, K = a.K, pitch = teacher_pitch(K);
   int64_t y;
@@ -541,6 +548,7 @@ __device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, int32_
     }
     tp[k] = p;
   }
+  wave_sync();
   E = wave_sum(E);
   bool label = false;  // among the pairs
   int32_t* place = a.place + r * (K + 1);
@@ -603,8 +611,10 @@ template <int DT, int PHASE, int T, int NC, int U, int WPE = 1> static int run_l
 // Threads a row by its pieces.  The step holds the row in as few registers a thread as the threads allow, with as few
 // rows in flight as keep the memory busy: the bf16 step of 8192 x 32000 takes 201 us with four workgroups of 512
 // threads on a compute unit, 189 us with two of 1024; that of 4096 x 50257 189 us with one workgroup of 1024 threads
-// and 100 registers, 164 us with two in 64 registers (waves a SIMD as the last argument); 4096 x 65536 230 us and, by
-// two of 512 threads, 206 us; 2048 x 130000 244 us held and 257 us read twice.
+// and 100 registers, 164 us with two in 64 registers (waves a SIMD as the last argument; with a teacher these spill,
+// 216 us, and two of 512 threads take 183); 4096 x 65536 230 us and, by two of 512 threads, 206 us; 2048 x 130000 244
+// us held and 257 us read twice.  Forward and backward are within 4 % of these for 256 to 1024 threads and two to six
+// pieces in flight, but for the backward, which 512 threads take 3 % longer.
 template <int DT, int PHASE> static int run_loss(const LossArgs& a, hipStream_t s) {
   const int pieces = a.V / Vec<DT>::N;
   if constexpr (PHASE == LOSS_STEP) {
@@ -643,6 +653,7 @@ bool loss_has_teacher(const LossArgs& a) { return a.sw != 0.f; }
 int launch_loss_prepare(const LossArgs& a, float* inv_count, hipStream_t s) {
   if (a.rows > 0 && loss_has_teacher(a)) {
     const unsigned blocks = (unsigned)((a.rows + TEACHER_ROWS - 1) / TEACHER_ROWS) + (inv_count ? 1 : 0);
+    if ((int64_t)blocks * TEACHER_ROWS * 64 > 0xffffffffll) return -2;  // a grid's threads are counted in 32 bits
     hipLaunchKernelGGL(loss_teacher_kernel, dim3(blocks), dim3(TEACHER_ROWS * 64), 8 * TEACHER_ROWS * teacher_pitch(a.K), s, a,
                        inv_count);
   } else if (inv_count) {
