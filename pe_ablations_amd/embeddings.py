@@ -11,9 +11,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .functional import _dtype_code, _on, _ptr, _stream, plain_autograd
+from .functional import _call, _ptr, _stream, plain_autograd
 
-_FLOATS = (torch.bfloat16, torch.float32, torch.float16)
+_FLOATS = {torch.bfloat16: _lib.PE_DTYPE_BF16, torch.float32: _lib.PE_DTYPE_FP32, torch.float16: _lib.PE_DTYPE_FP16}
 _INTS = (torch.int64, torch.int32)
 _MAX_TOKENS = 1 << 24
 
@@ -55,26 +55,23 @@ def _lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tens
     out = torch.empty(ids.shape + (H,), dtype=weight.dtype, device=dev)
     n = ids.numel()
     if n:
-        with _on(dev):
-            rc = _lib.lib().pe_embed_fwd(ids.data_ptr(), ids.element_size(), n, weight.data_ptr(),
-                                         _dtype_code(weight.dtype), V, H, max(weight.stride(0), H), scale, out.data_ptr(), H,
-                                         _stream(dev))
-        _lib.check(rc)
+        _call(dev, _lib.lib().pe_embed_fwd, ids.data_ptr(), ids.element_size(), n, weight.data_ptr(),
+              _FLOATS[weight.dtype], V, H, max(weight.stride(0), H), scale, out.data_ptr(), H, _stream(dev))
     return out
 
 
 def _gradient(ids: torch.Tensor, dy: torch.Tensor, V: int, scale: float, pad: int) -> torch.Tensor:
     """embedding_backward on checked arguments (pad: -1 for none)."""
     H, n, dev = dy.shape[-1], ids.numel(), dy.device
-    dy, ids = _rows(dy.reshape(-1, H), H), ids.contiguous()
+    if dy.dim() != 2:
+        dy = dy.reshape(-1, H)
+    dy, ids = _rows(dy, H), ids.contiguous()
     dw = torch.empty((V, H), dtype=dy.dtype, device=dev)
     L = _lib.lib()
     nb = L.pe_embed_bwd_workspace_bytes(n, V, H)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None  # held until the launch is enqueued
-    with _on(dev):
-        rc = L.pe_embed_bwd(ids.data_ptr(), ids.element_size(), n, dy.data_ptr(), _dtype_code(dy.dtype),
-                            max(dy.stride(0), H), V, H, scale, pad, dw.data_ptr(), H, _ptr(ws), nb, _stream(dev))
-    _lib.check(rc)
+    _call(dev, L.pe_embed_bwd, ids.data_ptr(), ids.element_size(), n, dy.data_ptr(), _FLOATS[dy.dtype],
+          max(dy.stride(0), H), V, H, scale, pad, dw.data_ptr(), H, _ptr(ws), nb, _stream(dev))
     return dw
 
 

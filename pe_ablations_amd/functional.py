@@ -188,6 +188,17 @@ def _on(dev: torch.device):
     return torch.cuda.device(dev)
 
 
+def _call(dev: torch.device, fn, *args) -> None:
+    """One library call with dev, a device of a CUDA tensor, current; raises what it returns."""
+    if dev.index == _current_device():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc:
+        _lib.check(rc)
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -659,18 +670,25 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
     return y.view(*x.shape[:-1], n)
 
 
+_functorch, _forward_ad = torch._C._functorch, torch.autograd.forward_ad
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_compiling = torch.compiler.is_compiling
+_PLAIN_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
 def plain_autograd(*tensors: torch.Tensor) -> bool:
     """Whether ordinary eager autograd is all that looks at these tensors, so that one fused Function may
     stand for a chain of torch ops: plain CUDA tensors, no functorch transform (vmap, jvp, grad), no
     batched gradients (is_grads_batched runs the backward under the older vmap), no forward-mode level, no
     tracing or compiling, and no dispatch or function mode that would see the ops."""
-    return (not torch.compiler.is_compiling()  # first: a compiler traces nothing of the rest
-            and all(t.is_cuda and type(t) in (torch.Tensor, torch.nn.Parameter)
-                    and not torch._C._functorch.is_legacy_batchedtensor(t) for t in tensors)
-            and torch._C._functorch.peek_interpreter_stack() is None
-            and torch.autograd.forward_ad._current_level < 0
-            and torch._C._len_torch_dispatch_stack() == 0 and torch._C._len_torch_function_stack() == 0
-            and not torch.jit.is_tracing())
+    if (_compiling()  # first: a compiler traces nothing of the rest
+            or _functorch.peek_interpreter_stack() is not None or _forward_ad._current_level >= 0
+            or _dispatch_modes() or _function_modes() or torch.jit.is_tracing()):
+        return False
+    for t in tensors:
+        if not t.is_cuda or type(t) not in _PLAIN_TENSORS or _functorch.is_legacy_batchedtensor(t):
+            return False
+    return True
 
 
 def rms_norm_expression(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:

@@ -31,9 +31,9 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .functional import _dtype_code, _expression_grads, _on, _ptr, _stream, plain_autograd
+from .functional import _call, _expression_grads, _ptr, _stream, plain_autograd
 
-_FLOATS = (torch.bfloat16, torch.float32, torch.float16)
+_FLOATS = {torch.bfloat16: _lib.PE_DTYPE_BF16, torch.float32: _lib.PE_DTYPE_FP32, torch.float16: _lib.PE_DTYPE_FP16}
 _INTS = (torch.int64, torch.int32)
 _REDUCTION = {"none": _lib.PE_LOSS_NONE, "sum": _lib.PE_LOSS_SUM, "mean": _lib.PE_LOSS_MEAN}
 
@@ -66,7 +66,7 @@ def _prepare(what, logits, labels, teacher_ids, teacher_logits, temperature, sof
     if x.stride(1) != 1 or x.stride(0) < V:
         x = x.contiguous()
     p = _lib.PeLossParams()
-    p.rows, p.vocab, p.dtype = x.shape[0], V, _dtype_code(x.dtype)
+    p.rows, p.vocab, p.dtype = x.shape[0], V, _FLOATS[x.dtype]
     p.row_stride, p.grad_row_stride = max(x.stride(0), V), V
     p.shift = lead[-1] if shift else 0
     p.ignore_index = ignore_index
@@ -91,7 +91,7 @@ def _prepare(what, logits, labels, teacher_ids, teacher_logits, temperature, sof
         if not 1e-3 <= temperature <= 1e3:
             raise ValueError(f"{what}: temperature must be in [0.001, 1000], got {temperature}")
         teacher_ids, teacher_logits = tid.reshape(-1, K).contiguous(), tlog.detach().reshape(-1, K).contiguous()
-        p.top_k, p.teacher_dtype, p.teacher_id_bytes = K, _dtype_code(tlog.dtype), tid.element_size()
+        p.top_k, p.teacher_dtype, p.teacher_id_bytes = K, _FLOATS[tlog.dtype], tid.element_size()
         p.teacher_id_stride = p.teacher_row_stride = K
         p.temperature = temperature
     return p, x, labels, teacher_ids, teacher_logits
@@ -107,10 +107,9 @@ def _forward(p, x, labels, tid, tlog, keep):
     n = L.pe_loss_stats_floats(ref) if keep else 0
     nb = L.pe_loss_workspace_bytes(ref)
     buf = torch.empty(n + nb // 4, dtype=torch.float32, device=dev)
-    with _on(dev):
-        rc = L.pe_loss_fwd(ref, x.data_ptr(), _ptr(labels), _ptr(tid), _ptr(tlog), loss.data_ptr(),
-                           buf.data_ptr() if keep else None, buf.data_ptr() + 4 * n, nb, _stream(dev))
-    _lib.check(rc)
+    at = buf.data_ptr()
+    _call(dev, L.pe_loss_fwd, ref, x.data_ptr(), _ptr(labels), _ptr(tid), _ptr(tlog), loss.data_ptr(),
+          at if keep else None, at + 4 * n, nb, _stream(dev))
     return loss, buf
 
 
@@ -169,13 +168,12 @@ class LossFn(torch.autograd.Function):
             return _expression_grads(lambda: _expression(logits, lab, rows(tid), rows(tlog), *ctx.args), (logits,), ctx,
                                      dloss) + (None,) * 5
         p = ctx.p
-        dz = torch.empty((p.rows, p.vocab), dtype=x.dtype, device=x.device)
+        dev = x.device
+        dz = torch.empty(logits.shape, dtype=x.dtype, device=dev)
         g = dloss.contiguous()
-        with _on(x.device):
-            rc = _lib.lib().pe_loss_bwd(ctypes.byref(p), x.data_ptr(), _ptr(lab), _ptr(tid), _ptr(tlog), buf.data_ptr(),
-                                        g.data_ptr(), dz.data_ptr(), _stream(x.device))
-        _lib.check(rc)
-        return (dz.view(logits.shape),) + (None,) * 5
+        _call(dev, _lib.lib().pe_loss_bwd, ctypes.byref(p), x.data_ptr(), _ptr(lab), _ptr(tid), _ptr(tlog),
+              buf.data_ptr(), g.data_ptr(), dz.data_ptr(), _stream(dev))
+        return (dz,) + (None,) * 5
 
 
 def _loss(what, logits, labels, teacher_ids, teacher_logits, temperature, soft_weight, ignore_index, reduction, shift):
@@ -241,9 +239,7 @@ def loss_and_grad(logits: torch.Tensor, labels: Optional[torch.Tensor], *, teach
     nb = L.pe_loss_workspace_bytes(ref)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    dz = torch.empty((p.rows, p.vocab), dtype=x.dtype, device=dev)
-    with _on(dev):
-        rc = L.pe_loss_step(ref, x.data_ptr(), _ptr(lab), _ptr(tid), _ptr(tlog), _ptr(scale), loss.data_ptr(),
-                            dz.data_ptr(), ws.data_ptr(), nb, _stream(dev))
-    _lib.check(rc)
-    return loss, dz.view(logits.shape)
+    dz = torch.empty(logits.shape, dtype=x.dtype, device=dev)
+    _call(dev, L.pe_loss_step, ref, x.data_ptr(), _ptr(lab), _ptr(tid), _ptr(tlog), _ptr(scale), loss.data_ptr(),
+          dz.data_ptr(), ws.data_ptr(), nb, _stream(dev))
+    return loss, dz
