@@ -308,17 +308,17 @@ struct LossArgs {
   int32_t* place;         // the teacher's rows: [rows][K + 1] ids and probabilities, [rows][2] sums
   float *prob, *tsum;
   float* row_loss;        // one per row
-  float* stats;           // [rows][3]: maximum, sum, sum at the temperature; [3 rows]: 1 / rows that count
+  float* stats;           // [rows][3]: maximum, sum, sum at the temperature; [3 rows]: the rows that count
   const float* dloss;     // one, or one per row (PE_LOSS_NONE)
-  const float* inv_count; // 1 / rows that count (PE_LOSS_MEAN)
+  const float* count;     // the rows that count (PE_LOSS_MEAN)
 };
 enum { LOSS_FWD = 0, LOSS_BWD = 1, LOSS_STEP = 2 };
 int launch_loss(int dtype, int phase, LossArgs a, hipStream_t s);
-// the teacher's rows, and 1 / rows that count (PE_LOSS_MEAN) from the labels unless inv_count is NULL
-int launch_loss_prepare(const LossArgs& a, float* inv_count, hipStream_t s);
+// the teacher's rows, and the number of rows that count unless `count` is NULL
+int launch_loss_prepare(const LossArgs& a, float* count, hipStream_t s);
 bool loss_has_teacher(const LossArgs& a);
-// the sum or mean of row_loss; also 1 / rows that count when inv_count is not NULL
-int launch_loss_reduce(const LossArgs& a, float* loss, float* inv_count, hipStream_t s);
+// the sum or mean of row_loss over `count`, which is formed here as well on request
+int launch_loss_reduce(const LossArgs& a, float* loss, float* count, bool form_count, hipStream_t s);
 
 // The scaled token embedding and its gradient
 struct EmbedArgs {

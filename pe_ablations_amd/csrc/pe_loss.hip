@@ -12,6 +12,8 @@
 // Bound by memory: one read of the logits forward, one read and one write backward, and one of each in the step, whose
 // workgroup holds its row in registers.  Rows are read in 16-byte pieces from the first 16-byte address on; the up
 // to seven elements on either side of the pieces are a thread's each.
+#include <type_traits>
+
 #include "pe_common.h"
 #include "pe_internal.h"
 #include "pe_vocab.h"
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
 
   float c = a.factor;
   if (a.dloss) c *= a.dloss[a.reduction == PE_LOSS_NONE ? r : 0];
-  if (a.inv_count) c *= *a.inv_count;
+  if (a.count) c /= *a.count;
   if (bad) c = NAN;
   float ch = 0.f, ct = 0.f;
   if (has_hard(MODE)) ch = c * a.hw / st.s;
@@ -440,63 +442,66 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
   if (!BWD) row_loss();
 }
 
-// 1 / rows that count, and the sum or mean of the row losses (SUM), by one workgroup of T threads, thread t taking rows
-// t, t + T, ..., the loads of U rows in flight.
-template <bool SUM, int T> __device__ __forceinline__ void reduce_rows(const LossArgs& a, float* loss, float* inv_count) {
-  __shared__ double rs[T / 64];
-  __shared__ int32_t rn[T / 64];
-  const int t = threadIdx.x;
-  double s = 0.;
-  int32_t n = 0;
-  const uint32_t rows = (uint32_t)a.rows, w = (uint32_t)a.label_bytes / 4, shift = (uint32_t)a.shift;
-  const int32_t* lab = (const int32_t*)a.labels;
+// The sum of the row losses in fp64 and the number of rows that count, by one workgroup of T threads, U rows a thread in
+// flight.  The rows that count are the labels other than ignore_index, but with `shift` the first of every sequence,
+// which is no row's.  L: the labels' type, or void for a sum alone.
+template <bool SUM, int T, class L> __device__ __forceinline__ void add_rows(const LossArgs& a, double& s, int32_t& n) {
+  constexpr bool COUNT = !std::is_void<L>::value;
+  using Y = typename std::conditional<COUNT, L, int32_t>::type;
+  const Y* lab = (const Y*)a.labels;
+  const uint32_t rows = (uint32_t)a.rows, shift = (uint32_t)a.shift;
   constexpr int U = 8;
-  for (uint32_t r0 = t; r0 < rows; r0 += U * T) {
+  for (uint32_t r0 = threadIdx.x; r0 < rows; r0 += U * T) {
     float x[U];
-    int32_t lo[U], hi[U];
-    bool last[U];
+    Y y[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t r = min(r0 + u * T, rows - 1);
       x[u] = SUM ? a.row_loss[r] : 0.f;
-      last[u] = shift && (r + 1) % shift == 0;
-      const uint64_t i = (uint64_t)(shift && !last[u] ? r + 1 : r) * w;
-      lo[u] = lab ? lab[i] : 0;
-      hi[u] = lab ? lab[i + w - 1] : 0;
+      y[u] = COUNT ? lab[r] : 0;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t y = w == 2 ? (int64_t)((uint64_t)(uint32_t)hi[u] << 32 | (uint32_t)lo[u]) : (int64_t)lo[u];
-      if (r0 + u * T < rows) {
-        s += x[u];
-        n += !lab || (!last[u] && y != a.ignore) ? 1 : 0;
-      }
+      const uint32_t r = r0 + u * T;
+      s += r < rows ? x[u] : 0.f;
+      n += COUNT && r < rows && (int64_t)y[u] != a.ignore && !(shift && r % shift == 0) ? 1 : 0;
     }
   }
+}
+template <bool SUM, bool COUNT, int T> __device__ __forceinline__ void reduce_rows(const LossArgs& a, float* loss, float* count) {
+  __shared__ double rs[T / 64];
+  __shared__ int32_t rn[T / 64];
+  double s = 0.;
+  int32_t n = 0;
+  if (COUNT && a.labels && a.label_bytes == 8) add_rows<SUM, T, int64_t>(a, s, n);
+  else if (COUNT && a.labels) add_rows<SUM, T, int32_t>(a, s, n);
+  else if (SUM) add_rows<SUM, T, void>(a, s, n);
+  if (!a.labels && threadIdx.x == 0) n = (int32_t)a.rows;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     if (SUM) s += __shfl_xor(s, o, 64);
-    n += __shfl_xor(n, o, 64);
+    if (COUNT) n += __shfl_xor(n, o, 64);
   }
-  if ((t & 63) == 0) {
-    rs[t >> 6] = s;
-    rn[t >> 6] = n;
+  if ((threadIdx.x & 63) == 0) {
+    rs[threadIdx.x >> 6] = s;
+    rn[threadIdx.x >> 6] = n;
   }
   __syncthreads();
-  if (t != 0) return;
+  if (threadIdx.x != 0) return;
   for (int i = 1; i < T / 64; ++i) {
     s += rs[i];
     n += rn[i];
   }
-  if (SUM) *loss = (float)(a.reduction == PE_LOSS_MEAN ? s / (double)n : s);
-  if (inv_count) *inv_count = 1.f / (float)n;
+  if (COUNT) *count = (float)n;
+  if (SUM) *loss = (float)(a.reduction == PE_LOSS_MEAN ? s / (COUNT ? (double)n : (double)*count) : s);
 }
 
-__global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* loss, float* inv_count) {
-  reduce_rows<true, 1024>(a, loss, inv_count);
+__global__ __launch_bounds__(1024) void loss_count_kernel(LossArgs a, float* count) {
+  reduce_rows<false, true, 1024>(a, nullptr, count);
 }
-__global__ __launch_bounds__(1024) void loss_count_kernel(LossArgs a, float* inv_count) {
-  reduce_rows<false, 1024>(a, nullptr, inv_count);
+// the count is formed here (COUNT) or was ahead of the rows
+template <bool COUNT> __global__ __launch_bounds__(1024) void loss_reduce_kernel(LossArgs a, float* loss, float* count) {
+  reduce_rows<true, COUNT, 1024>(a, loss, count);
 }
 
 // The teacher's pairs, ahead of the rows' workgroups, which would wait for them: a wave takes a row.  What the rows need
@@ -515,9 +520,8 @@ __device__ __forceinline__ void wave_sync() {
 
 __device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, int32_t* tid, float* tp) {
   const int lane = threadIdx.x & 63, K = a.K, pitch = teacher_pitch(K);
-  int64_t y;
-  if (!row_label(a, (uint32_t)r, y)) return;
-  if (!a.labels || a.hw == 0.f || y < 0 || y >= a.V) y = -1;
+  int64_t y;  // on its way beside the pairs; a row that does not count is not waited for
+  const bool counts = row_label(a, (uint32_t)r, y);
   const float lt = LOG2E / a.T;
   float mx = -INFINITY;
   for (int k = lane; k < pitch; k += 64) {
@@ -550,6 +554,7 @@ __device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, int32_
   }
   wave_sync();
   E = wave_sum(E);
+  if (!counts || !a.labels || a.hw == 0.f || y < 0 || y >= a.V) y = -1;
   bool label = false;  // among the pairs
   int32_t* place = a.place + r * (K + 1);
   float* prob = a.prob + r * (K + 1);
@@ -583,12 +588,12 @@ __device__ __forceinline__ void teacher_row(const LossArgs& a, int64_t r, int32_
   }
 }
 
-// the teacher's rows; with inv_count also the number of rows that count, by a workgroup ahead of them
-__global__ __launch_bounds__(TEACHER_ROWS * 64) void loss_teacher_kernel(LossArgs a, float* inv_count) {
+// the teacher's rows; with `count` also the number of rows that count, by a workgroup ahead of them
+__global__ __launch_bounds__(TEACHER_ROWS * 64) void loss_teacher_kernel(LossArgs a, float* count) {
   extern __shared__ __attribute__((aligned(16))) char dyn[];
   int64_t block = blockIdx.x;
-  if (inv_count && block-- == 0) {
-    reduce_rows<false, TEACHER_ROWS * 64>(a, nullptr, inv_count);
+  if (count && block-- == 0) {
+    reduce_rows<false, true, TEACHER_ROWS * 64>(a, nullptr, count);
     return;
   }
   const int w = threadIdx.x >> 6, pitch = teacher_pitch(a.K);
@@ -650,20 +655,21 @@ int launch_loss(int dtype, int phase, LossArgs a, hipStream_t s) {
 
 bool loss_has_teacher(const LossArgs& a) { return a.sw != 0.f; }
 
-int launch_loss_prepare(const LossArgs& a, float* inv_count, hipStream_t s) {
+int launch_loss_prepare(const LossArgs& a, float* count, hipStream_t s) {
   if (a.rows > 0 && loss_has_teacher(a)) {
-    const unsigned blocks = (unsigned)((a.rows + TEACHER_ROWS - 1) / TEACHER_ROWS) + (inv_count ? 1 : 0);
+    const unsigned blocks = (unsigned)((a.rows + TEACHER_ROWS - 1) / TEACHER_ROWS) + (count ? 1 : 0);
     if ((int64_t)blocks * TEACHER_ROWS * 64 > 0xffffffffll) return -2;  // a grid's threads are counted in 32 bits
     hipLaunchKernelGGL(loss_teacher_kernel, dim3(blocks), dim3(TEACHER_ROWS * 64), 8 * TEACHER_ROWS * teacher_pitch(a.K), s, a,
-                       inv_count);
-  } else if (inv_count) {
-    hipLaunchKernelGGL(loss_count_kernel, dim3(1), dim3(1024), 0, s, a, inv_count);
+                       count);
+  } else if (count) {
+    hipLaunchKernelGGL(loss_count_kernel, dim3(1), dim3(1024), 0, s, a, count);
   }
   return hipGetLastError() == hipSuccess ? 0 : -7;
 }
 
-int launch_loss_reduce(const LossArgs& a, float* loss, float* inv_count, hipStream_t s) {
-  hipLaunchKernelGGL(loss_reduce_kernel, dim3(1), dim3(1024), 0, s, a, loss, inv_count);
+int launch_loss_reduce(const LossArgs& a, float* loss, float* count, bool form_count, hipStream_t s) {
+  if (form_count) hipLaunchKernelGGL(loss_reduce_kernel<true>, dim3(1), dim3(1024), 0, s, a, loss, count);
+  else hipLaunchKernelGGL(loss_reduce_kernel<false>, dim3(1), dim3(1024), 0, s, a, loss, count);
   return hipGetLastError() == hipSuccess ? 0 : -7;
 }
 

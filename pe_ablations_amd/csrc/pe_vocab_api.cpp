@@ -115,7 +115,7 @@ int pe_loss_check(const pe_loss_params* p) {
 }
 
 size_t pe_loss_workspace_bytes(const pe_loss_params* p) {
-  // the row losses, 1 / rows that count, the teacher's rows
+  // the row losses, the number of rows that count, the teacher's rows
   return pe_loss_check(p) ? 0 : (size_t)(p->rows + 1 + teacher_floats(p)) * 4;
 }
 
@@ -137,7 +137,7 @@ int pe_loss_fwd(const pe_loss_params* p, const void* logits, const void* labels,
   set_teacher(a, stats ? stats + 3 * p->rows + 1 : (float*)workspace + p->rows + 1);
   if ((rc = pe::launch_loss_prepare(a, nullptr, (hipStream_t)stream))) return rc;
   if ((rc = pe::launch_loss(p->dtype, pe::LOSS_FWD, a, (hipStream_t)stream)) || !whole) return rc;
-  return pe::launch_loss_reduce(a, loss, stats ? stats + 3 * p->rows : nullptr, (hipStream_t)stream);
+  return pe::launch_loss_reduce(a, loss, stats ? stats + 3 * p->rows : (float*)workspace + p->rows, true, (hipStream_t)stream);
 }
 
 int pe_loss_bwd(const pe_loss_params* p, const void* logits, const void* labels, const void* teacher_ids,
@@ -153,7 +153,7 @@ int pe_loss_bwd(const pe_loss_params* p, const void* logits, const void* labels,
   a.stats = const_cast<float*>(stats);
   set_teacher(a, a.stats + 3 * p->rows + 1);
   a.dloss = dloss;
-  a.inv_count = p->reduction == PE_LOSS_MEAN ? stats + 3 * p->rows : nullptr;
+  a.count = p->reduction == PE_LOSS_MEAN ? stats + 3 * p->rows : nullptr;
   return pe::launch_loss(p->dtype, pe::LOSS_BWD, a, (hipStream_t)stream);
 }
 
@@ -172,11 +172,11 @@ int pe_loss_step(const pe_loss_params* p, const void* logits, const void* labels
   a.row_loss = (float*)workspace;
   a.dloss = grad_scale;
   set_teacher(a, (float*)workspace + p->rows + 1);
-  float* inv = p->reduction == PE_LOSS_MEAN ? (float*)workspace + p->rows : nullptr;
-  if ((rc = pe::launch_loss_prepare(a, inv, (hipStream_t)stream))) return rc;
-  a.inv_count = inv;
+  float* count = p->reduction == PE_LOSS_MEAN ? (float*)workspace + p->rows : nullptr;
+  if ((rc = pe::launch_loss_prepare(a, count, (hipStream_t)stream))) return rc;
+  a.count = count;
   if ((rc = pe::launch_loss(p->dtype, pe::LOSS_STEP, a, (hipStream_t)stream))) return rc;
-  return pe::launch_loss_reduce(a, loss, nullptr, (hipStream_t)stream);
+  return pe::launch_loss_reduce(a, loss, count, false, (hipStream_t)stream);
 }
 
 }  // extern "C"
