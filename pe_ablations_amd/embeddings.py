@@ -138,6 +138,8 @@ class TokenEmbedding(nn.Module):
     """``scale`` (an addition; default None = the reference's plain lookup through torch): the rows times this
     factor, sqrt(embed_dim) in models that tie the weight to an output projection, through ``embedding``."""
 
+    scale: Optional[float] = None  # also of a module pickled without one
+
     def __init__(self, vocab_size: int, embed_dim: int, scale: Optional[float] = None):
         super().__init__()
         self.vocab_size = vocab_size

@@ -16,6 +16,9 @@ gives every row's loss (its negative is the token's log probability).  ``shift=T
 labels (..., S) of the same positions and holds row s to label s + 1, without the shifted copy of the logits that
 slicing would make; the last row of each sequence does not count.
 
+At high temperatures the soft part is T^2 times a small difference of numbers near log V and keeps that many digits
+fewer (about 1e-4 absolute at T = 10); its gradient does not suffer.
+
 Everything is computed in fp32 from bf16, fp16 or fp32 logits, losses are fp32, gradients are rounded once to the
 logits' dtype; sums run in a fixed order.  The differentiable forms keep the logits for their backward, so these must
 not be changed in place in between (autograd notices).  Where something other than plain autograd looks at the logits

@@ -154,3 +154,47 @@ def test_graph_replay(cuda):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b), rep
+
+
+@pytest.mark.parametrize("n", [700, 5000])
+def test_two_graphs(cuda, n):
+    """Two captured graphs, replayed in turn with eager work between them: neither touches the other's workspace; both
+    forms of the embedding's gradient."""
+    g = torch.Generator(device=cuda).manual_seed(n)
+
+    def make(V, H, dtype):
+        w = torch.randn(V, H, generator=g, device=cuda).to(dtype).requires_grad_(True)
+        ids = torch.randint(0, V, (n,), generator=g, device=cuda)
+        dy = torch.randn(n, H, generator=g, device=cuda).to(dtype)
+        z = torch.randn(60, V, generator=g, device=cuda).to(dtype)
+        y = torch.randint(0, V, (60,), generator=g, device=cuda)
+        tid, tlog = torch.randint(0, V, (60, 6), generator=g, device=cuda), torch.randn(60, 6, generator=g, device=cuda)
+
+        def step():
+            (dw,) = torch.autograd.grad(embedding(ids, w, scale=2.0), w, dy)
+            loss, dz = loss_and_grad(z, y, teacher_ids=tid, teacher_logits=tlog, temperature=2.0)
+            return dw, loss, dz, cross_entropy(z, y, reduction="none")
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        return step, graph, outs
+
+    both = [make(2000, 40, torch.float32), make(901, 72, torch.bfloat16)]
+    want = [[t.clone() for t in step()] for step, _, _ in both]
+    for rep in range(4):
+        for step, graph, outs in both[::-1] if rep % 2 else both:
+            for t in outs:
+                t.fill_(float("nan"))
+            graph.replay()
+            step()
+        torch.cuda.synchronize()
+        for (_, _, outs), w in zip(both, want):
+            for a, b in zip(outs, w):
+                assert torch.equal(a, b), rep
