@@ -7,9 +7,11 @@
 // the run of every row of the vocabulary: each row of the gradient is written once, by one workgroup, rows without a
 // token as zeros, and no sum depends on the order in which workgroups run.
 //
-// A row of H elements is cut into pieces of VB bytes, the largest of 16, 8, 4 and 2 that the row length, the strides
-// and the addresses allow, a piece a lane; `lpr` lanes (a power of two) work on a row together, 256 / lpr rows at
-// once in a workgroup, and rows longer than lpr pieces are cut into column slices.
+// A row of H elements is cut into pieces, a piece a lane: 16 bytes where the row length, the strides and the addresses
+// are multiples of 16; else 16 bytes at any address, the last piece moved back to end with the row (its elements that
+// the piece before has as well are worked out twice, to the same values); single elements in rows below 16 bytes.
+// `lpr` lanes (a power of two) work on a row together, 256 / lpr rows at once in a workgroup, and rows longer than lpr
+// pieces are cut into column slices.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,26 +22,25 @@ namespace pe {
 
 namespace {
 
-template <int VB> struct Raw;
-template <> struct Raw<16> { using T = u32x4; };
-template <> struct Raw<8> { using T = u32x2; };
-template <> struct Raw<4> { using T = uint32_t; };
-template <> struct Raw<2> { using T = uint16_t; };
+enum { ELEMENT = 0, ALIGNED = 1, ANYWHERE = 2 };
 
-// a piece of VB bytes of a row of dtype DT as floats
-template <int DT, int VB> struct Piece {
-  static constexpr int ES = DT == 1 ? 4 : 2, N = VB / ES;
-  using R = typename Raw<VB>::T;
-  static __device__ __forceinline__ R load(const void* p, int64_t byte) { return *(const R*)((const char*)p + byte); }
+// a piece of a row of dtype DT as floats
+template <int DT, int KIND> struct Piece {
+  static constexpr int ES = DT == 1 ? 4 : 2, N = KIND == ELEMENT ? 1 : 16 / ES;
+  using R = typename std::conditional<KIND != ELEMENT, u32x4,
+                                      typename std::conditional<DT == 1, uint32_t, uint16_t>::type>::type;
+  using M = typename std::conditional<KIND == ANYWHERE, u32x4_any, R>::type;  // as it lies in memory
+  // the first element of piece c
+  static __device__ __forceinline__ int first(const EmbedArgs& a, int c) { return KIND == ANYWHERE ? min(c * N, a.H - N) : c * N; }
+  static __device__ __forceinline__ R load(const void* p, int64_t byte) { return *(const M*)((const char*)p + byte); }
   static __device__ __forceinline__ void unpack(const R& r, float (&x)[N]) {
-    if constexpr (VB == 2) {
-      x[0] = DT == 0 ? bf2f(r) : h2f(r);
+    if constexpr (KIND == ELEMENT) {
+      if constexpr (DT == 1) x[0] = __builtin_bit_cast(float, r);
+      else x[0] = DT == 0 ? bf2f(r) : h2f(r);
     } else {
 #pragma unroll
-      for (int i = 0; i < VB / 4; ++i) {
-        uint32_t w;
-        if constexpr (VB == 4) w = r;
-        else w = r[i];
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = r[i];
         if constexpr (DT == 1) x[i] = __builtin_bit_cast(float, w);
         else if constexpr (DT == 0) {
           x[2 * i] = __builtin_bit_cast(float, w << 16);
@@ -52,23 +53,21 @@ template <int DT, int VB> struct Piece {
   }
   static __device__ __forceinline__ void store(void* p, int64_t byte, const float (&x)[N], bool stream) {
     R r;
-    if constexpr (VB == 2) {
-      r = DT == 0 ? f2bf(x[0]) : f2h(x[0]);
+    if constexpr (KIND == ELEMENT) {
+      if constexpr (DT == 1) r = __builtin_bit_cast(uint32_t, x[0]);
+      else r = DT == 0 ? f2bf(x[0]) : f2h(x[0]);
     } else {
 #pragma unroll
-      for (int i = 0; i < VB / 4; ++i) {
-        uint32_t w;
-        if constexpr (DT == 1) w = __builtin_bit_cast(uint32_t, x[i]);
-        else if constexpr (DT == 0) w = pack_bf2(x[2 * i], x[2 * i + 1]);
-        else w = pack_h2(x[2 * i], x[2 * i + 1]);
-        if constexpr (VB == 4) r = w;
-        else r[i] = w;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == 1) r[i] = __builtin_bit_cast(uint32_t, x[i]);
+        else if constexpr (DT == 0) r[i] = pack_bf2(x[2 * i], x[2 * i + 1]);
+        else r[i] = pack_h2(x[2 * i], x[2 * i + 1]);
       }
     }
-    R* q = (R*)((char*)p + byte);
+    M* q = (M*)((char*)p + byte);
     if (stream) {
       asm volatile("");  // on either side: else the compiler makes one plain store of the two
-      __builtin_nontemporal_store(r, q);
+      __builtin_nontemporal_store((M)r, q);
       asm volatile("");
     } else {
       *q = r;
@@ -93,18 +92,19 @@ __device__ __forceinline__ float product(float x, float s) {
 // ------------------------------------------------------------------ lookup
 constexpr int LOOKUP_ROWS = 4;  // rows a group of lanes has in flight
 
-template <int DT, int VB> __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a) {
-  using P = Piece<DT, VB>;
+template <int DT, int KIND> __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a) {
+  using P = Piece<DT, KIND>;
   const int sub = threadIdx.x & (a.lpr - 1), grp = threadIdx.x / a.lpr, ng = 256 / a.lpr;
   const int64_t t0 = ((int64_t)blockIdx.x * ng + grp) * LOOKUP_ROWS;
   int64_t id[LOOKUP_ROWS];
 #pragma unroll
   for (int i = 0; i < LOOKUP_ROWS; ++i) id[i] = t0 + i < a.n ? load_id(a.ids, a.id_bytes, t0 + i) : -1;
   for (int c = sub; c < a.pieces; c += a.lpr) {
+    const int j = P::first(a, c);
     typename P::R r[LOOKUP_ROWS] = {};
 #pragma unroll
     for (int i = 0; i < LOOKUP_ROWS; ++i)
-      if (id[i] >= 0 && id[i] < a.V) r[i] = P::load(a.x, id[i] * a.x_rs * P::ES + (int64_t)c * VB);
+      if (id[i] >= 0 && id[i] < a.V) r[i] = P::load(a.x, (id[i] * a.x_rs + j) * P::ES);
 #pragma unroll
     for (int i = 0; i < LOOKUP_ROWS; ++i) {
       if (t0 + i >= a.n) break;
@@ -112,7 +112,7 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_fwd_kerne
       P::unpack(r[i], x);
 #pragma unroll
       for (int e = 0; e < P::N; ++e) x[e] = id[i] >= 0 && id[i] < a.V ? product(x[e], a.scale) : NAN;
-      P::store(a.y, (t0 + i) * a.y_rs * P::ES + (int64_t)c * VB, x, a.stream);
+      P::store(a.y, ((t0 + i) * a.y_rs + j) * P::ES, x, a.stream);
     }
   }
 }
@@ -260,9 +260,9 @@ __global__ __launch_bounds__(TILE) void embed_scatter_kernel(EmbedArgs a, SortAr
 
 // ------------------------------------------------------------------ sums of rows
 // Rows first, first + 1, ... of a list, added in order with `U` loads in flight
-template <int DT, int VB, int U = 8, class F>
-__device__ __forceinline__ void add_rows(const void* x, int64_t col, int64_t first, int64_t end, F row, float (&s)[Piece<DT, VB>::N]) {
-  using P = Piece<DT, VB>;
+template <int DT, int KIND, int U = 8, class F>
+__device__ __forceinline__ void add_rows(const void* x, int64_t col, int64_t first, int64_t end, F row, float (&s)[Piece<DT, KIND>::N]) {
+  using P = Piece<DT, KIND>;
   int64_t i = first;
   for (; i + U <= end; i += U) {
     typename P::R r[U];
@@ -285,8 +285,8 @@ __device__ __forceinline__ void add_rows(const void* x, int64_t col, int64_t fir
 }
 
 // the sums of chunks k, k + 1, ... behind one another, four of them in flight
-template <int N> __device__ __forceinline__ void add_sums(const EmbedArgs& a, int c, int32_t k, int32_t end, float (&s)[N]) {
-  const float* p = a.part + (int64_t)c * N;
+template <int N> __device__ __forceinline__ void add_sums(const EmbedArgs& a, int j, int32_t k, int32_t end, float (&s)[N]) {
+  const float* p = a.part + j;
   for (; k + 4 <= end; k += 4) {
     float x[4][N];
 #pragma unroll
@@ -305,8 +305,8 @@ template <int N> __device__ __forceinline__ void add_sums(const EmbedArgs& a, in
 
 // A chunk of a.chunk sorted tokens: notes where runs begin and end in it, and if all of it has one id adds up its
 // rows, the workgroup's groups of lanes taking a run of tokens each and their sums added in order.
-template <int DT, int VB> __global__ __launch_bounds__(256) void embed_chunk_kernel(EmbedArgs a) {
-  using P = Piece<DT, VB>;
+template <int DT, int KIND> __global__ __launch_bounds__(256) void embed_chunk_kernel(EmbedArgs a) {
+  using P = Piece<DT, KIND>;
   const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;  // a row's slices side by side
   const int64_t c0 = (int64_t)bx * a.chunk, c1 = c0 + a.chunk;
   if (slice == 0) {
@@ -326,7 +326,7 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_chunk_ker
   float s[P::N] = {};
   const int64_t i0 = c0 + (int64_t)a.chunk * grp / ng, i1 = c0 + (int64_t)a.chunk * (grp + 1) / ng;
   if (c < a.pieces)
-    add_rows<DT, VB, 16>(a.x, (int64_t)c * VB, i0, i1, [&](int64_t i) { return (int64_t)a.order[i] * a.x_rs * P::ES; }, s);
+    add_rows<DT, KIND, 16>(a.x, (int64_t)P::first(a, c) * P::ES, i0, i1, [&](int64_t i) { return (int64_t)a.order[i] * a.x_rs * P::ES; }, s);
 #pragma unroll
   for (int e = 0; e < P::N; ++e) red[threadIdx.x * P::N + e] = s[e];
   __syncthreads();
@@ -335,7 +335,7 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_chunk_ker
 #pragma unroll
       for (int e = 0; e < P::N; ++e) s[e] += red[(g * a.lpr + sub) * P::N + e];
 #pragma unroll
-    for (int e = 0; e < P::N; ++e) a.part[(int64_t)bx * a.H + (int64_t)c * P::N + e] = s[e];
+    for (int e = 0; e < P::N; ++e) a.part[(int64_t)bx * a.H + P::first(a, c) + e] = s[e];
   }
 }
 
@@ -346,12 +346,13 @@ constexpr int MAX_ROWS = 64;   // rows of the vocabulary a workgroup takes
 // so are shared out.  Each group of lanes takes the rows with short runs in turn; then the workgroup adds up each long
 // run together, as the tokens ahead of its first whole chunk, the chunks' sums (CHUNKS), and the tokens behind the
 // last, cut into as many equal parts as there are groups, whose sums are added in order.
-template <int DT, int VB, bool CHUNKS, class O>
+template <int DT, int KIND, bool CHUNKS, class O>
 __device__ __forceinline__ void grad_rows(const EmbedArgs& a, int slice, int bx, int64_t G, int nr, const int2* run, float* red, O order) {
-  using P = Piece<DT, VB>;
+  using P = Piece<DT, KIND>;
   const int sub = threadIdx.x & (a.lpr - 1), grp = threadIdx.x / a.lpr, ng = 256 / a.lpr;
   const int c = slice * a.lpr + sub;
-  const int64_t col = (int64_t)c * VB;
+  const int j0 = P::first(a, c);
+  const int64_t col = (int64_t)j0 * P::ES;
   auto token = [&](int64_t i) { return (int64_t)order(i) * a.x_rs * P::ES; };
   auto put = [&](int j, float (&s)[P::N]) {
 #pragma unroll
@@ -363,7 +364,7 @@ __device__ __forceinline__ void grad_rows(const EmbedArgs& a, int slice, int bx,
       const int32_t i0 = run[j].x, i1 = run[j].y;
       if (i1 - i0 > SHORT_RUN) continue;
       float s[P::N] = {};
-      add_rows<DT, VB, 4>(a.x, col, i0, i1, token, s);
+      add_rows<DT, KIND, 4>(a.x, col, i0, i1, token, s);
       put(j, s);
     }
   }
@@ -378,11 +379,11 @@ __device__ __forceinline__ void grad_rows(const EmbedArgs& a, int slice, int bx,
     const int32_t b0 = (int32_t)((int64_t)total * grp / ng), b1 = (int32_t)((int64_t)total * (grp + 1) / ng);
     float s[P::N] = {};
     if (c < a.pieces) {
-      add_rows<DT, VB>(a.x, col, i0 + min(b0, h), i0 + min(b1, h), token, s);
+      add_rows<DT, KIND>(a.x, col, i0 + min(b0, h), i0 + min(b1, h), token, s);
       if (chunks) {
-        add_sums<P::N>(a, c, k0 + min(max(b0 - h, 0), m), k0 + min(max(b1 - h, 0), m), s);
+        add_sums<P::N>(a, j0, k0 + min(max(b0 - h, 0), m), k0 + min(max(b1 - h, 0), m), s);
         const int64_t q = (int64_t)k1 * a.chunk - h - m;  // item b behind the chunks is token q + b
-        add_rows<DT, VB>(a.x, col, q + max(b0, h + m), q + max(b1, h + m), token, s);
+        add_rows<DT, KIND>(a.x, col, q + max(b0, h + m), q + max(b1, h + m), token, s);
       }
     }
     __syncthreads();
@@ -401,16 +402,16 @@ __device__ __forceinline__ void grad_rows(const EmbedArgs& a, int slice, int bx,
 // Bound by the latency of the tokens' rows, so by how many waves a SIMD holds and how many workgroups there are (bf16
 // 32000 x 2048, 16384 / 65536 tokens, the whole gradient: 69 / 124 us with eight rows in flight in 87 registers and
 // 1024 workgroups, 58 / 115 us with four in 64, 58 / 112 us with 2048 workgroups, 65 / 114 us with 4096).
-template <int DT, int VB>
+template <int DT, int KIND>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void embed_bwd_kernel(EmbedArgs a) {
   const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;
   __shared__ int2 run[MAX_ROWS];
-  __shared__ float red[256 * Piece<DT, VB>::N];
+  __shared__ float red[256 * Piece<DT, KIND>::N];
   const int64_t G = gridDim.x / a.slices;
   const int nr = (int)((a.V - bx + G - 1) / G);
   if (threadIdx.x < nr) run[threadIdx.x] = a.run[bx + threadIdx.x * G];
   __syncthreads();
-  grad_rows<DT, VB, true>(a, slice, bx, G, nr, run, red, [&](int64_t i) { return a.order[i]; });
+  grad_rows<DT, KIND, true>(a, slice, bx, G, nr, run, red, [&](int64_t i) { return a.order[i]; });
 }
 
 // Up to FEW tokens, in one launch without a workspace: every workgroup picks the tokens of its own rows from all of them
@@ -418,8 +419,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void e
 // row's in turn.
 constexpr int FEW = 4096;
 
-template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_few_kernel(EmbedArgs a, int log_g) {
-  constexpr int N = Piece<DT, VB>::N;
+template <int DT, int KIND> __global__ __launch_bounds__(256) void embed_bwd_few_kernel(EmbedArgs a, int log_g) {
+  constexpr int N = Piece<DT, KIND>::N;
   const int slice = blockIdx.x % a.slices, bx = blockIdx.x / a.slices;
   __shared__ int2 run[MAX_ROWS];
   __shared__ uint16_t order[FEW];
@@ -477,30 +478,28 @@ template <int DT, int VB> __global__ __launch_bounds__(256) void embed_bwd_few_k
     if (lane == 0) run[j] = int2{before, before + len};
   }
   __syncthreads();
-  grad_rows<DT, VB, false>(a, slice, bx, G, nr, run, u.red, [&](int64_t i) { return (int32_t)order[i]; });
+  grad_rows<DT, KIND, false>(a, slice, bx, G, nr, run, u.red, [&](int64_t i) { return (int32_t)order[i]; });
 }
 
 namespace {
 
-// the bytes a lane takes of a row: the most that the row's length, its strides and its addresses are multiples of
-int piece_bytes(int es, const EmbedArgs& a) {
+int piece_kind(int es, const EmbedArgs& a) {
   const uint64_t all = (uint64_t)(uintptr_t)a.x | (uintptr_t)a.y | (uint64_t)(a.x_rs * es) | (uint64_t)(a.y_rs * es) |
                        (uint64_t)((int64_t)a.H * es);
-  for (int vb = 16; vb > es; vb /= 2)
-    if (all % vb == 0) return vb;
-  return es;
+  return all % 16 == 0 ? ALIGNED : ((int64_t)a.H * es >= 16 ? ANYWHERE : ELEMENT);
 }
+int pieces_of(int kind, int H, int es) { return kind == ELEMENT ? H : (int)(((int64_t)H * es + 15) / 16); }
 
-template <class F> int with_piece(int dtype, int vb, F&& f) {
+template <class F> int with_piece(int dtype, int kind, F&& f) {
   using std::integral_constant;
-  auto go = [&](auto dt, auto v) { return f(dt, v); };
-#define PE_PIECE(D, B) \
-  if (dtype == D && vb == B) return go(integral_constant<int, D>{}, integral_constant<int, B>{})
-  PE_PIECE(0, 16); PE_PIECE(0, 8); PE_PIECE(0, 4); PE_PIECE(0, 2);
-  PE_PIECE(1, 16); PE_PIECE(1, 8); PE_PIECE(1, 4);
-  PE_PIECE(2, 16); PE_PIECE(2, 8); PE_PIECE(2, 4); PE_PIECE(2, 2);
-#undef PE_PIECE
-  return -4;
+  auto go = [&](auto dt) {
+    if (kind == ALIGNED) return f(dt, integral_constant<int, ALIGNED>{});
+    if (kind == ANYWHERE) return f(dt, integral_constant<int, ANYWHERE>{});
+    return f(dt, integral_constant<int, ELEMENT>{});
+  };
+  if (dtype == 0) return go(integral_constant<int, 0>{});
+  if (dtype == 1) return go(integral_constant<int, 1>{});
+  return go(integral_constant<int, 2>{});
 }
 
 // lanes a row: the power of two that covers its pieces, from 8 up to `most`
@@ -539,14 +538,14 @@ int done() { return hipGetLastError() == hipSuccess ? 0 : -7; }
 }  // namespace
 
 int launch_embed_fwd(int dtype, EmbedArgs a, hipStream_t s) {
-  const int es = dtype == 1 ? 4 : 2, vb = piece_bytes(es, a);
-  a.pieces = (int)((int64_t)a.H * es / vb);
+  const int es = dtype == 1 ? 4 : 2, kind = piece_kind(es, a);
+  a.pieces = pieces_of(kind, a.H, es);
   a.lpr = lanes_per_row(a.pieces, 256);
   a.stream = streams(a.n, a.H, es);
   const int64_t rows = (int64_t)(256 / a.lpr) * LOOKUP_ROWS;
   const dim3 grid((unsigned)((a.n + rows - 1) / rows)), block(256);
   if (!grid_fits((a.n + rows - 1) / rows, 256)) return -2;
-  return with_piece(dtype, vb, [&](auto dt, auto v) {
+  return with_piece(dtype, kind, [&](auto dt, auto v) {
     hipLaunchKernelGGL((embed_fwd_kernel<decltype(dt)::value, decltype(v)::value>), grid, block, 0, s, a);
     return done();
   });
@@ -559,8 +558,8 @@ int64_t embed_bwd_workspace(int64_t n, int64_t V, int H) {
 }
 
 int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s) {
-  const int es = dtype == 1 ? 4 : 2, vb = piece_bytes(es, a);
-  a.pieces = (int)((int64_t)a.H * es / vb);
+  const int es = dtype == 1 ? 4 : 2, kind = piece_kind(es, a);
+  a.pieces = pieces_of(kind, a.H, es);
   // Lanes on a row: a whole workgroup where most rows of the gradient are zeros, so that the tokens are picked for
   // all of its columns at once; else a wave, whose slices and groups share the long runs (fp32 50257 x 512, 4096
   // tokens: 29 against 37 us; bf16 2000 x 1024, 4096 tokens: 24 against 18 us)
@@ -572,7 +571,7 @@ int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s) {
     int log_g = 0;
     while (((int64_t)15 << (log_g + 1)) <= a.V || (log_g < 9 && ((int64_t)2 << log_g) <= a.V)) ++log_g;
     if (!grid_fits((int64_t)a.slices << log_g, 256)) return -2;
-    return with_piece(dtype, vb, [&](auto dt, auto v) {
+    return with_piece(dtype, kind, [&](auto dt, auto v) {
       hipLaunchKernelGGL((embed_bwd_few_kernel<decltype(dt)::value, decltype(v)::value>), dim3((unsigned)a.slices << log_g),
                          dim3(256), 0, s, a, log_g);
       return done();
@@ -609,7 +608,7 @@ int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s) {
   const unsigned rows = (unsigned)((a.V + MAX_ROWS - 1) / MAX_ROWS);
   const unsigned grid = (unsigned)std::min<int64_t>(a.V, std::max<int64_t>(rows, 2048));
   if (!grid_fits((int64_t)std::max(grid, chunks) * a.slices, 256)) return -2;
-  return with_piece(dtype, vb, [&](auto dt, auto v) {
+  return with_piece(dtype, kind, [&](auto dt, auto v) {
     constexpr int D = decltype(dt)::value, B = decltype(v)::value;
     hipLaunchKernelGGL((embed_chunk_kernel<D, B>), dim3(chunks * a.slices), dim3(256), 0, s, a);
     hipLaunchKernelGGL((embed_bwd_kernel<D, B>), dim3(grid * a.slices), dim3(256), 0, s, a);

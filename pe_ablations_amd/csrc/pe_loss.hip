@@ -108,20 +108,16 @@ template <int DT> struct Row {
     return NT ? __builtin_nontemporal_load(q) : *q;
   }
 };
-// piece k of the gradient's row: 16 bytes where its rows are aligned as the logits' are, else element by element
-enum { STORE_ELEMENTS, STORE_PLAIN, STORE_STREAM };
-template <int DT> __device__ __forceinline__ void store_piece(char* body, int k, int how, const float (&x)[Vec<DT>::N]) {
-  u32x4* q = (u32x4*)(body + (uint32_t)k * 16u);
-  if (how == STORE_STREAM) {
-    const u32x4 r = Vec<DT>::pack(x);
+// piece k of the gradient's row, whose rows need not be aligned as the logits' are
+template <int DT> __device__ __forceinline__ void store_piece(char* body, int k, bool stream, const float (&x)[Vec<DT>::N]) {
+  u32x4_any* q = (u32x4_any*)(body + (uint32_t)k * 16u);
+  const u32x4 r = Vec<DT>::pack(x);
+  if (stream) {
     asm volatile("");  // on either side: else the compiler makes one plain store of the two
-    __builtin_nontemporal_store(r, q);
+    __builtin_nontemporal_store((u32x4_any)r, q);
     asm volatile("");
-  } else if (how == STORE_PLAIN) {
-    *q = Vec<DT>::pack(x);
   } else {
-#pragma unroll
-    for (int e = 0; e < Vec<DT>::N; ++e) put<DT>(q, e, x[e]);
+    *q = r;
   }
 }
 
@@ -225,12 +221,11 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
   const Row<DT> row(z, V);
   char* const dbody = FWD ? nullptr : dz + row.head * W::ES;
   const int one = row.single(t);
-  const int how = ((uintptr_t)z ^ (uintptr_t)dz) & 15 ? STORE_ELEMENTS : (a.stream ? STORE_STREAM : STORE_PLAIN);
   int64_t y;
   if (!row_label(a, (uint32_t)r, y)) {
     if (!FWD) {
       const float zero[N] = {};
-      for (int k = t; k < row.nvec; k += T) store_piece<DT>(dbody, k, how, zero);
+      for (int k = t; k < row.nvec; k += T) store_piece<DT>(dbody, k, a.stream, zero);
       if (one >= 0) put<DT>(dz, one, 0.f);
     }
     if (t == 0) {
@@ -406,7 +401,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(WPE))) void l
     W::unpack(raw, x);
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = dense(x[e]);
-    store_piece<DT>(dbody, k, how, x);
+    store_piece<DT>(dbody, k, a.stream, x);
   };
   if (one >= 0) put<DT>(dz, one, dense(xone));
   if (NC > 0) {
