@@ -527,7 +527,8 @@ int key_bits(int64_t V) {  // of keys 0 .. V
 }
 
 // Outputs beyond this size are stored past the 256 MB cache, smaller ones left in it for their reader (the gradient of
-// 32000 x 2048 in bf16, 125 MB: 58 and 48 us; of 50257 x 512 in fp32, 98 MB: 44 and 47 us).
+// 32000 x 2048 in bf16, 125 MB, 16384 tokens: 58 and 48 us; of 50257 x 512 in fp32, 98 MB: 44 and 47 us).  The gradient of
+// a few tokens, nearly all zeros, never is (the former with 2048 tokens: 32 us streamed, 29 us not).
 bool streams(int64_t rows, int H, int es) { return rows * H * es > (112ll << 20); }
 
 // a grid's threads are counted in 32 bits
@@ -565,7 +566,7 @@ int launch_embed_bwd(int dtype, EmbedArgs a, void* ws, hipStream_t s) {
   // tokens: 29 against 37 us; bf16 2000 x 1024, 4096 tokens: 24 against 18 us)
   a.lpr = lanes_per_row(a.pieces, a.n <= FEW && a.V >= 4 * a.n ? 256 : 64);
   a.slices = (a.pieces + a.lpr - 1) / a.lpr;
-  a.stream = streams(a.V, a.H, es);
+  a.stream = a.n > FEW && streams(a.V, a.H, es);
   if (a.n <= FEW) {
     // 15 to 30 rows a workgroup, fewer where that leaves compute units idle
     int log_g = 0;
